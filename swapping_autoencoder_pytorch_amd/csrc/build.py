@@ -8,6 +8,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 OUT = os.path.join(HERE, "libsae_hip.so")
 ARCH = "gfx950"
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): hipcc makes them out of ordinary float code by itself, and some of their
+# forms have given wrong results now and then (the host pass does not know the feature and says so: harmless)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def sources():
@@ -24,7 +27,7 @@ def includes():
 
 
 def deps():
-    return sources() + includes() + [os.path.join(HERE, "sae_common.h"), os.path.join(ROOT, "include", "sae_hip.h")]
+    return sources() + includes() + [os.path.join(HERE, "sae_common.h"), os.path.join(ROOT, "include", "sae_hip.h"), os.path.join(HERE, "build.py")]
 
 
 def up_to_date():
@@ -39,8 +42,8 @@ def hipcc():
 
 
 def _source_deps(src):
-    """What one source is rebuilt for: itself, the two headers, and -- for the file that #includes them -- the .inc parts."""
-    d = [src, os.path.join(HERE, "sae_common.h"), os.path.join(ROOT, "include", "sae_hip.h")]
+    """What one source is rebuilt for: itself, the two headers, the flags here, and -- for the file that #includes them -- the .inc parts."""
+    d = [src, os.path.join(HERE, "sae_common.h"), os.path.join(ROOT, "include", "sae_hip.h"), os.path.join(HERE, "build.py")]
     with open(src) as f:
         if ".inc\"" in f.read():
             d += includes()
@@ -54,7 +57,7 @@ def compile_and_link(out, objdir, extra_flags=(), force=False, verbose=False, jo
     cc = hipcc()
     os.makedirs(objdir, exist_ok=True)
     flags = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-I", os.path.join(ROOT, "include"),
-             "-I", HERE] + list(extra_flags)
+             "-I", HERE] + NO_PACKED_FP32 + list(extra_flags)
     todo, objs = [], []
     for src in sources():
         obj = os.path.join(objdir, os.path.basename(src) + ".o")

@@ -9,6 +9,6 @@ src=$C/s2wino.hip
 if [ -n "$1" ] && [ "${1#-}" = "$1" ]; then src=$1; shift; fi
 others=$(ls $C/build/product/*.o | grep -v s2wino.hip.o)
 mkdir -p tools/variants
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-value -I include -I $C "$@" -c $src -o /tmp/s2w_$name.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -Wno-unused-value -I include -I $C "$@" -c $src -o /tmp/s2w_$name.o
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC /tmp/s2w_$name.o $others -o tools/variants/$name.so
 echo built tools/variants/$name.so
