@@ -60,7 +60,7 @@
 extern "C" {
 #endif
 
-#define SAE_ABI_VERSION 12  /* 12: sae_s2wino_* (stride-2 3x3 family on the polyphase minimal-filtering form);  11: sae_gemm_ws_f32 (K split across workgroups);  10: sae_adam_multi_dev_f32 (step counts in device memory: hipGraph replays);  9: sae_wino_fused_wgrad_*;  8: sae_wino_fused_* (one-kernel Winograd convolution);  7: sae_wino_* (Winograd F(2x2,3x3) transforms);  6: prepared weights (sae_conv2d_desc::prepped*, sae_conv2d_wprep_*);  2: modconv / adam / glue entry points (round 2), 3: sae_upfirdn2d_epilogue_f32, 4: sae_conv2d_fwd_residual_f32, 5: sae_weight_demod_*, sae_modconv2d_fwd_noise_bias_act_f32, sae_upfirdn2d_noise_bias_act_f32, sae_plane_scale_dot_act_f32 */
+#define SAE_ABI_VERSION 13  /* 13: sae_group_norm_act*, sae_checkpoint8_*, sae_linear_wgrad8 (channels-last normalisation, 8-bit activation checkpoints);  12: sae_s2wino_* (stride-2 3x3 family on the polyphase minimal-filtering form);  11: sae_gemm_ws_f32 (K split across workgroups);  10: sae_adam_multi_dev_f32 (step counts in device memory: hipGraph replays);  9: sae_wino_fused_wgrad_*;  8: sae_wino_fused_* (one-kernel Winograd convolution);  7: sae_wino_* (Winograd F(2x2,3x3) transforms);  6: prepared weights (sae_conv2d_desc::prepped*, sae_conv2d_wprep_*);  2: modconv / adam / glue entry points (round 2), 3: sae_upfirdn2d_epilogue_f32, 4: sae_conv2d_fwd_residual_f32, 5: sae_weight_demod_*, sae_modconv2d_fwd_noise_bias_act_f32, sae_upfirdn2d_noise_bias_act_f32, sae_plane_scale_dot_act_f32 */
 
 #define SAE_OK 0
 #define SAE_EINVAL (-1)    /* bad argument (null pointer, non-positive size, unsupported mode) */
@@ -508,6 +508,53 @@ int sae_s2wino_weights_f32(const float* w, const float* row_scale, const float* 
                            int64_t w_stride_out, int64_t w_stride_in, int32_t flip, float alpha, sae_stream_t stream);
 int sae_s2wino_dgrad_f32(const float* g, const float* g_scale, const float* uf, const float* out_scale, float* dx, int64_t n,
                          int64_t cin, int64_t cout, int64_t h, int64_t w, sae_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Channels-last operators in three element types.  The reference has none of them: they stand beside its bias + activation and
+ * linear layers for networks that normalise and for steps whose activations are kept in 8 bits.  All arithmetic is fp32 or wider.
+ */
+#define SAE_F32 0
+#define SAE_BF16 1
+#define SAE_F16 2
+#define SAE_ACT_NONE 0
+#define SAE_ACT_LRELU 1    /* z > 0 ? z : slope * z */
+#define SAE_ACT_SILU 2     /* z / (1 + exp(-z)) */
+
+/* 8-bit activation checkpoints (csrc/checkpoint8.hip).  A row x [c] is cut into blocks of 32 values (the last one may be short);
+ * a block has one step 2^k, the least exponent with max |x| <= 127.5 * 2^k (-126 <= k <= 121; SAE_F16: -24 <= k <= 9), and stands
+ * for q * 2^k with q = x / 2^k rounded to the nearest (ties to even) in [-127, 127], where a value that is not zero never gets q = 0.
+ * A block with a NaN or an infinity stands for NaN.
+ *   codes   [rows][32 * blocks], blocks = ceil(c / 32), zero behind the row's last value; 16-byte aligned
+ *   scales  [blocks][rows]: k + 127 (255: NaN)
+ * sae_checkpoint8_pack writes both, sae_checkpoint8_unpack gives the values in the element type. */
+int sae_checkpoint8_pack(const void* x, int8_t* codes, uint8_t* scales, int64_t rows, int64_t c, int32_t dtype,
+                         sae_stream_t stream);
+int sae_checkpoint8_unpack(const int8_t* codes, const uint8_t* scales, void* x, int64_t rows, int64_t c, int32_t dtype,
+                           sae_stream_t stream);
+
+/* Group normalisation + activation on x [n][l][c] (csrc/group_norm.hip): statistics over the l * (c / groups) values of a sample's
+ * group, z = (x - mean) * rstd * weight[c] + bias[c] (either may be NULL: 1, 0), y = scale * act(z).
+ *   sae_group_norm_act      writes y, mean and rstd [n][groups], and -- if given -- the 8-bit checkpoint of x (rows = n * l)
+ *   sae_group_norm_act_bwd  from gy and EITHER x OR its checkpoint: gx [n][l][c], gw and gb [c] (any of the three may be NULL; with
+ *                           n * l = 0 gw and gb are zero).  From a checkpoint the gradients are those at the values it stands for,
+ *                           with the statistics of the forward pass.
+ *   sae_group_norm_act_workspace   bytes of workspace either needs (backward = 0 / 1)
+ * Tensors and workspace 16-byte aligned, n <= 65535.  Sums are added in a fixed order (no atomics). */
+int64_t sae_group_norm_act_workspace(int64_t n, int64_t l, int64_t c, int64_t groups, int32_t dtype, int32_t backward);
+int sae_group_norm_act(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd, int8_t* codes,
+                       uint8_t* scales, int64_t n, int64_t l, int64_t c, int64_t groups, float eps, int32_t act, float slope,
+                       float scale, int32_t dtype, void* workspace, int64_t workspace_bytes, sae_stream_t stream);
+int sae_group_norm_act_bwd(const void* gy, const void* x, const int8_t* codes, const uint8_t* scales, const float* mean,
+                           const float* rstd, const float* weight, const float* bias, void* gx, float* gw, float* gb, int64_t n,
+                           int64_t l, int64_t c, int64_t groups, int32_t act, float slope, float scale, int32_t dtype,
+                           void* workspace, int64_t workspace_bytes, sae_stream_t stream);
+
+/* Weight gradient of a linear layer from its input's 8-bit checkpoint (csrc/linear_wgrad8.hip):
+ *   gw[o][i] = alpha * sum over r of gy[r][o] * x8[r][i]   [out][c],     gb[o] = sum over r of gy[r][o]   (gb may be NULL)
+ * gy, gw, gb in the element type; products exact, sums fp32.  workspace: sae_linear_wgrad8_workspace floats, 16-byte aligned. */
+int64_t sae_linear_wgrad8_workspace(int64_t rows, int64_t out, int64_t c);
+int sae_linear_wgrad8(const void* gy, const int8_t* codes, const uint8_t* scales, void* gw, void* gb, int64_t rows, int64_t out,
+                      int64_t c, float alpha, int32_t dtype, float* workspace, int64_t workspace_floats, sae_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -42,7 +42,7 @@ typedef struct sae_conv2d_desc {
 
 static __thread char g_err[256];
 
-int oracle_abi_version(void) { return 12; }
+int oracle_abi_version(void) { return 13; }
 const char* oracle_last_error(void) { return g_err; }
 
 /* include/sae_hip.h: the mode only selects GPU arithmetic; the oracle always accumulates in double */
@@ -1463,5 +1463,219 @@ int oracle_s2wino_dgrad_f32(const float* g, const float* g_scale, const float* u
             }
             free(V);
         }
+    return SAE_OK;
+}
+
+/* ------------------------------------------------------------------------------------------------------------------------------
+ * Channels-last operators and 8-bit activation checkpoints (include/sae_hip.h).  The reference has none: restated here from the
+ * definitions, element by element in double, and pinned by the tests to torch's double-precision autograd of the same formulas.
+ */
+static double el_get(const void* p, int64_t i, int32_t dtype) {
+    if (dtype == 0) return ((const float*)p)[i];
+    const uint16_t h = ((const uint16_t*)p)[i];
+    if (dtype == 1) {
+        const uint32_t u = (uint32_t)h << 16;
+        float f;
+        memcpy(&f, &u, 4);
+        return f;
+    }
+    const int s = h >> 15, e = (h >> 10) & 31, m = h & 1023;
+    double v;
+    if (e == 31) v = m ? NAN : INFINITY;
+    else if (e == 0) v = ldexp(m, -24);
+    else v = ldexp(1024 + m, e - 25);
+    return s ? -v : v;
+}
+/* v rounded to `bits` significant bits, exponent of the last place at least `least`; ties to even */
+static double round_bits(double v, int bits, int least) {
+    if (v == 0.0 || !isfinite(v)) return v;
+    int e;
+    frexp(v, &e);
+    int ulp = e - bits;
+    if (ulp < least) ulp = least;
+    return ldexp(nearbyint(ldexp(v, -ulp)), ulp);
+}
+static void el_put(void* p, int64_t i, int32_t dtype, double v) {
+    if (dtype == 0) {
+        ((float*)p)[i] = (float)v;
+        return;
+    }
+    uint16_t h;
+    const uint16_t s = signbit(v) ? 0x8000 : 0;
+    if (dtype == 1) {
+        float f = (float)round_bits(v, 8, -133);
+        uint32_t u;
+        memcpy(&u, &f, 4);
+        h = isnan(v) ? 0x7fc0 : (uint16_t)(u >> 16);
+    } else if (isnan(v)) {
+        h = 0x7e00;
+    } else {
+        const double r = fabs(round_bits(v, 11, -24));
+        int e;
+        if (r >= 65520.0) h = s | 0x7c00;
+        else if (r < ldexp(1, -14)) h = s | (uint16_t)ldexp(r, 24);
+        else {
+            const double m = frexp(r, &e);           /* r = m 2^e, m in [0.5, 1) */
+            h = s | (uint16_t)((e + 14) << 10) | (uint16_t)(ldexp(m, 11) - 1024);
+        }
+    }
+    ((uint16_t*)p)[i] = h;
+}
+
+int oracle_checkpoint8_pack(const void* x, int8_t* codes, uint8_t* scales, int64_t rows, int64_t c, int32_t dtype,
+                            sae_stream_t stream) {
+    (void)stream;
+    if (dtype < 0 || dtype > 2 || rows < 0 || c < 1 || (rows > 0 && (!x || !codes || !scales)))
+        return set_err("oracle_checkpoint8_pack: bad argument");
+    const int64_t blocks = (c + 31) / 32;
+    for (int64_t r = 0; r < rows; ++r)
+        for (int64_t b = 0; b < blocks; ++b) {
+            double top = 0.0;
+            int bad = 0;
+            for (int64_t i = 32 * b; i < 32 * b + 32 && i < c; ++i) {
+                const double v = fabs(el_get(x, r * c + i, dtype));
+                if (!isfinite(v)) bad = 1;
+                else if (v > top) top = v;
+            }
+            int k = dtype == 2 ? -24 : -126;
+            while (k < (dtype == 2 ? 9 : 121) && top > ldexp(127.5, k)) ++k;
+            scales[b * rows + r] = bad ? 255 : (uint8_t)(k + 127);
+            for (int64_t i = 32 * b; i < 32 * b + 32; ++i) {
+                double q = 0.0;
+                if (i < c && !bad) {
+                    const double v = el_get(x, r * c + i, dtype);
+                    q = nearbyint(ldexp(v, -k));
+                    if (q > 127) q = 127;
+                    if (q < -127) q = -127;
+                    if (q == 0.0 && v != 0.0) q = v > 0 ? 1 : -1;
+                }
+                codes[r * blocks * 32 + i] = (int8_t)q;
+            }
+        }
+    return SAE_OK;
+}
+
+static double kept_get(const int8_t* codes, const uint8_t* scales, int64_t r, int64_t i, int64_t rows, int64_t blocks) {
+    const int e = scales[(i / 32) * rows + r];
+    return e == 255 ? NAN : ldexp(codes[r * blocks * 32 + i], e - 127);
+}
+
+int oracle_checkpoint8_unpack(const int8_t* codes, const uint8_t* scales, void* x, int64_t rows, int64_t c, int32_t dtype,
+                              sae_stream_t stream) {
+    (void)stream;
+    if (dtype < 0 || dtype > 2 || rows < 0 || c < 1 || (rows > 0 && (!x || !codes || !scales)))
+        return set_err("oracle_checkpoint8_unpack: bad argument");
+    for (int64_t r = 0; r < rows; ++r)
+        for (int64_t i = 0; i < c; ++i) el_put(x, r * c + i, dtype, kept_get(codes, scales, r, i, rows, (c + 31) / 32));
+    return SAE_OK;
+}
+
+static double act_value(double z, int32_t act, double slope) {
+    if (act == 1) return z > 0 ? z : slope * z;
+    return act == 2 ? z / (1.0 + exp(-z)) : z;
+}
+static double act_derivative(double z, int32_t act, double slope) {
+    if (act == 1) return z > 0 ? 1.0 : slope;
+    if (act != 2) return 1.0;
+    const double s = 1.0 / (1.0 + exp(-z));
+    return s * (1.0 + z * (1.0 - s));
+}
+
+int64_t oracle_group_norm_act_workspace(int64_t n, int64_t l, int64_t c, int64_t groups, int32_t dtype, int32_t backward) {
+    (void)n; (void)l; (void)c; (void)groups; (void)dtype; (void)backward;
+    return 16;
+}
+
+int oracle_group_norm_act(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd, int8_t* codes,
+                          uint8_t* scales, int64_t n, int64_t l, int64_t c, int64_t groups, float eps, int32_t act, float slope,
+                          float scale, int32_t dtype, void* workspace, int64_t workspace_bytes, sae_stream_t stream) {
+    (void)workspace; (void)workspace_bytes;
+    if (dtype < 0 || dtype > 2 || act < 0 || act > 2 || n < 0 || l < 0 || c < 1 || groups < 1 || c % groups || !(eps >= 0) || !codes != !scales)
+        return set_err("oracle_group_norm_act: bad argument");
+    const int64_t cg = c / groups;
+    for (int64_t i = 0; i < n && l > 0; ++i)
+        for (int64_t g = 0; g < groups; ++g) {
+            double s = 0.0, v = 0.0;
+            for (int64_t p = 0; p < l; ++p)
+                for (int64_t j = g * cg; j < (g + 1) * cg; ++j) s += el_get(x, (i * l + p) * c + j, dtype);
+            const double mu = s / ((double)l * cg);
+            for (int64_t p = 0; p < l; ++p)
+                for (int64_t j = g * cg; j < (g + 1) * cg; ++j) {
+                    const double d = el_get(x, (i * l + p) * c + j, dtype) - mu;
+                    v += d * d;
+                }
+            const double r = 1.0 / sqrt(v / ((double)l * cg) + (double)eps);
+            mean[i * groups + g] = (float)mu;
+            rstd[i * groups + g] = (float)r;
+            for (int64_t p = 0; p < l; ++p)
+                for (int64_t j = g * cg; j < (g + 1) * cg; ++j) {
+                    const int64_t at = (i * l + p) * c + j;
+                    const double z = (el_get(x, at, dtype) - mu) * r * (weight ? weight[j] : 1.0) + (bias ? bias[j] : 0.0);
+                    el_put(y, at, dtype, act_value(z, act, slope) * scale);
+                }
+        }
+    return codes ? oracle_checkpoint8_pack(x, codes, scales, n * l, c, dtype, stream) : SAE_OK;
+}
+
+int oracle_group_norm_act_bwd(const void* gy, const void* x, const int8_t* codes, const uint8_t* scales, const float* mean,
+                              const float* rstd, const float* weight, const float* bias, void* gx, float* gw, float* gb, int64_t n,
+                              int64_t l, int64_t c, int64_t groups, int32_t act, float slope, float scale, int32_t dtype,
+                              void* workspace, int64_t workspace_bytes, sae_stream_t stream) {
+    (void)workspace; (void)workspace_bytes; (void)stream;
+    if (dtype < 0 || dtype > 2 || act < 0 || act > 2 || n < 0 || l < 0 || c < 1 || groups < 1 || c % groups || !codes != !scales)
+        return set_err("oracle_group_norm_act_bwd: bad argument");
+    const int64_t cg = c / groups, blocks = (c + 31) / 32;
+    double* sums = (double*)calloc((size_t)(2 * c), sizeof(double));
+    for (int64_t i = 0; i < n && l > 0; ++i)
+        for (int64_t g = 0; g < groups; ++g) {
+            const double mu = mean[i * groups + g], r = rstd[i * groups + g];
+            double m1 = 0.0, m2 = 0.0;
+            for (int pass = 0; pass < 2; ++pass)
+                for (int64_t p = 0; p < l; ++p)
+                    for (int64_t j = g * cg; j < (g + 1) * cg; ++j) {
+                        const int64_t at = (i * l + p) * c + j;
+                        const double v = codes ? kept_get(codes, scales, i * l + p, j, n * l, blocks) : el_get(x, at, dtype);
+                        const double w = weight ? weight[j] : 1.0, xh = (v - mu) * r;
+                        const double dz = el_get(gy, at, dtype) * scale * act_derivative(xh * w + (bias ? bias[j] : 0.0), act, slope);
+                        if (pass == 0) {
+                            sums[j] += dz;
+                            sums[c + j] += dz * xh;
+                            m1 += w * dz / ((double)l * cg);
+                            m2 += w * dz * xh / ((double)l * cg);
+                        } else if (gx) {
+                            el_put(gx, at, dtype, r * (w * dz - m1 - xh * m2));
+                        }
+                    }
+        }
+    for (int64_t j = 0; j < c; ++j) {
+        if (gb) gb[j] = (float)sums[j];
+        if (gw) gw[j] = (float)sums[c + j];
+    }
+    free(sums);
+    return SAE_OK;
+}
+
+int64_t oracle_linear_wgrad8_workspace(int64_t rows, int64_t out, int64_t c) {
+    (void)rows; (void)out; (void)c;
+    return 4;
+}
+
+int oracle_linear_wgrad8(const void* gy, const int8_t* codes, const uint8_t* scales, void* gw, void* gb, int64_t rows, int64_t out,
+                         int64_t c, float alpha, int32_t dtype, float* workspace, int64_t workspace_floats, sae_stream_t stream) {
+    (void)workspace; (void)workspace_floats; (void)stream;
+    if (dtype < 0 || dtype > 2 || rows < 0 || out < 1 || c < 1 || !gw) return set_err("oracle_linear_wgrad8: bad argument");
+    double* row = (double*)calloc((size_t)c, sizeof(double));
+    for (int64_t o = 0; o < out; ++o) {
+        double b = 0.0;
+        for (int64_t i = 0; i < c; ++i) row[i] = 0.0;
+        for (int64_t r = 0; r < rows; ++r) {
+            const double g = el_get(gy, r * out + o, dtype);
+            b += g;
+            for (int64_t i = 0; i < c; ++i) row[i] += g * kept_get(codes, scales, r, i, rows, (c + 31) / 32);
+        }
+        for (int64_t i = 0; i < c; ++i) el_put(gw, o * c + i, dtype, alpha * row[i]);
+        if (gb) el_put(gb, o, dtype, b);
+    }
+    free(row);
     return SAE_OK;
 }

@@ -1,5 +1,6 @@
 """Build csrc/libsae_hip.so for gfx950 with hipcc (cross-compiles without a GPU)."""
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -41,13 +42,22 @@ def hipcc():
     raise RuntimeError("hipcc not found: cannot build the gfx950 hot-path library")
 
 
+def _included(src):
+    """The .inc parts a source #includes, directly or through another part (paths relative to csrc/)."""
+    found, todo = [], [src]
+    while todo:
+        with open(todo.pop()) as f:
+            for name in re.findall(r'#include "([\w/]+\.inc)"', f.read()):
+                path = os.path.join(HERE, name)
+                if path not in found and os.path.exists(path):
+                    found.append(path)
+                    todo.append(path)
+    return found
+
+
 def _source_deps(src):
-    """What one source is rebuilt for: itself, the two headers, the flags here, and -- for the file that #includes them -- the .inc parts."""
-    d = [src, os.path.join(HERE, "sae_common.h"), os.path.join(ROOT, "include", "sae_hip.h"), os.path.join(HERE, "build.py")]
-    with open(src) as f:
-        if ".inc\"" in f.read():
-            d += includes()
-    return d
+    """What one source is rebuilt for: itself, the two headers, the flags here, and the .inc parts it #includes."""
+    return [src, os.path.join(HERE, "sae_common.h"), os.path.join(ROOT, "include", "sae_hip.h"), os.path.join(HERE, "build.py")] + _included(src)
 
 
 def compile_and_link(out, objdir, extra_flags=(), force=False, verbose=False, jobs=None):

@@ -10,6 +10,7 @@ util/util.py:432-436, which raises on ROCm; that gate is not consulted here.)
 same signatures of the CPU oracle (``oracle_*``) and of the emulator build of the kernels
 (tests/emu) for checking; the product never does.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -43,7 +44,7 @@ class ConvMod(C.Structure):
     _fields_ = [("x_scale", C.c_void_p), ("y_scale", C.c_void_p), ("wm_scale", C.c_void_p), ("wc_scale", C.c_void_p)]
 
 
-ABI_VERSION = 12     # include/sae_hip.h: SAE_ABI_VERSION
+ABI_VERSION = 13     # include/sae_hip.h: SAE_ABI_VERSION
 
 _SIGNATURES = {
     "abi_version": (C.c_int, []),
@@ -124,6 +125,16 @@ _SIGNATURES = {
     "s2wino_weights_floats": (_i64, [_i64, _i64]),
     "s2wino_weights_f32": (C.c_int, [_f32p, _f32p, _f32p, _f32p, _i64, _i64, _i64, _i64, _i32, _f32, _stream]),
     "s2wino_dgrad_f32": (C.c_int, [_f32p, _f32p, _f32p, _f32p, _f32p, _i64, _i64, _i64, _i64, _i64, _stream]),
+    "checkpoint8_pack": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, _i64, _i64, _i32, _stream]),
+    "checkpoint8_unpack": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, _i64, _i64, _i32, _stream]),
+    "group_norm_act_workspace": (_i64, [_i64, _i64, _i64, _i64, _i32, _i32]),
+    "group_norm_act": (C.c_int, [C.c_void_p, _f32p, _f32p, C.c_void_p, _f32p, _f32p, C.c_void_p, C.c_void_p, _i64, _i64, _i64, _i64,
+                                 _f32, _i32, _f32, _f32, _i32, C.c_void_p, _i64, _stream]),
+    "group_norm_act_bwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, _f32p, _f32p, _f32p, _f32p, C.c_void_p, _f32p,
+                                     _f32p, _i64, _i64, _i64, _i64, _i32, _f32, _f32, _i32, C.c_void_p, _i64, _stream]),
+    "linear_wgrad8_workspace": (_i64, [_i64, _i64, _i64]),
+    "linear_wgrad8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, _i64, _i64, _i64, _f32, _i32, _f32p,
+                                _i64, _stream]),
 }
 
 EXPORTED_SYMBOLS = tuple("sae_" + name for name in _SIGNATURES)
@@ -191,6 +202,31 @@ class SaeLibrary:
                     "tensor on %s: the MI355X hot path has no CPU implementation (move the model "
                     "and data to a GPU)" % t.device)
 
+    def check_channels_last(self, *tensors):
+        """Tensors of the channels-last operators: f32, bf16 or f16, one type and one device for all, contiguous, 16-byte aligned
+        (`dense` makes them so) and (product) on a GPU."""
+        first = None
+        for t in tensors:
+            if t is None:
+                continue
+            if t.dtype not in element_types():
+                raise SaeError("channels-last kernels take float32, bfloat16 and float16, got %s" % t.dtype)
+            if first is not None and (t.dtype != first.dtype or t.device != first.device):
+                raise SaeError("tensors of one call must share type and device, got %s on %s and %s on %s"
+                               % (first.dtype, first.device, t.dtype, t.device))
+            if not t.is_contiguous() or t.data_ptr() % 16:
+                raise SaeError("internal error: non-contiguous or misaligned tensor reached the C-ABI")
+            if self.device_only and not t.is_cuda:
+                raise SaeError("tensor on %s: the MI355X operators have no CPU implementation" % t.device)
+            first = t if first is None else first
+
+    def device_of(self, t):
+        """Context in which launches go to the tensor's device: the default stream's handle says nothing about its device."""
+        import torch
+        if t.is_cuda and t.device.index != torch.cuda.current_device():
+            return torch.cuda.device(t.device)
+        return contextlib.nullcontext()
+
     def stream(self, t):
         """Raw handle of the CURRENT stream of the tensor's device (what the reference's ops launch on).  The raw query
         is one C call; `torch.cuda.current_stream(dev).cuda_stream` builds a Stream object per launch (5 us, 330 launches
@@ -217,6 +253,23 @@ def get():
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+_ELEMENT_TYPES = {}
+
+
+def element_types():
+    """torch type -> code of the channels-last entry points (include/sae_hip.h: SAE_F32 / SAE_BF16 / SAE_F16)."""
+    if not _ELEMENT_TYPES:
+        import torch
+        _ELEMENT_TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    return _ELEMENT_TYPES
+
+
+def dense(t):
+    """`t` contiguous and 16-byte aligned: itself where it is, a copy where not (a slice that starts inside a 16-byte cell)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 CONV_MATH_MODES = {"f32": 0, "bf16x6": 1}

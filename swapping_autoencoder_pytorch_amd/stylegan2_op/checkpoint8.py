@@ -1,0 +1,191 @@
+"""8-bit activation checkpoints: what a backward pass needs of the forward pass, kept in a quarter (f32) or half (bf16, f16) of
+its size, and the operators that read it there (csrc/checkpoint8.hip, csrc/linear_wgrad8.hip).
+
+The format (csrc/elem8.inc): blocks of 32 values along the last dimension with one power-of-two step each and a signed 8-bit code
+for each value; an error of at most half a step, 2^-8 ... 2^-7 of the block's largest value, where only a zero becomes zero (what
+is smaller than half a step becomes one step), so sign(x) is exact -- the mask that a leaky ReLU's backward reads.  (Next to the
+type's largest number, above 127.5 steps of the largest step, the error is up to one step.)  A block with a
+NaN or an infinity comes back as NaN.
+
+  checkpoint8               activation -> Checkpoint8, ``.dequantize()`` gives it back
+  linear_weight_grad8       weight and bias gradient of a linear layer from the Checkpoint8 of its input
+  linear8                   ``linear`` that keeps its input as a Checkpoint8
+  activation_checkpoints8   every node built inside keeps the activations it saves as Checkpoint8s
+
+The reference keeps every activation in fp32 (it never enables AMP)."""
+import contextlib
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from .. import hip_lib
+from .conv2d_gemm import _Flags, _gemm
+
+BLOCK = 32
+
+
+class Checkpoint8:
+    """codes int8 [rows, 32 * blocks] (zero behind a row's last value), scales uint8 [blocks, rows] (exponent of the step + 127,
+    255: NaN), blocks = ceil(channels / 32); stands for a tensor of ``shape`` (default [rows, channels]) and ``dtype``."""
+    __slots__ = ("codes", "scales", "channels", "dtype", "shape")
+
+    def __init__(self, codes, scales, channels, dtype, shape=None):
+        blocks = -(-channels // BLOCK)
+        if channels < 1 or dtype not in hip_lib.element_types():
+            raise hip_lib.SaeError("Checkpoint8: channels >= 1 and float32 / bfloat16 / float16, got %d, %s" % (channels, dtype))
+        if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] != BLOCK * blocks or not codes.is_contiguous():
+            raise hip_lib.SaeError("Checkpoint8: codes must be contiguous int8 [rows, %d], got %s %s"
+                                   % (BLOCK * blocks, codes.dtype, tuple(codes.shape)))
+        if scales.dtype != torch.uint8 or tuple(scales.shape) != (blocks, codes.shape[0]) or not scales.is_contiguous():
+            raise hip_lib.SaeError("Checkpoint8: scales must be contiguous uint8 %s, got %s %s"
+                                   % ((blocks, codes.shape[0]), scales.dtype, tuple(scales.shape)))
+        if codes.device != scales.device:
+            raise hip_lib.SaeError("Checkpoint8: codes on %s, scales on %s" % (codes.device, scales.device))
+        shape = torch.Size((codes.shape[0], channels) if shape is None else shape)
+        if not shape or shape[-1] != channels or shape[:-1].numel() != codes.shape[0]:
+            raise hip_lib.SaeError("Checkpoint8: shape %s is not %d rows of %d" % (tuple(shape), codes.shape[0], channels))
+        self.codes, self.scales, self.channels, self.dtype, self.shape = hip_lib.dense(codes), scales, channels, dtype, shape
+
+    @property
+    def rows(self):
+        return self.codes.shape[0]
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def dequantize(self):
+        """The values the codes stand for, a new contiguous tensor."""
+        lib = hip_lib.get()
+        x = torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
+        lib.check_channels_last(x)
+        with lib.device_of(x):
+            lib.call("checkpoint8_unpack", self.codes.data_ptr(), self.scales.data_ptr(), x.data_ptr(), self.rows, self.channels,
+                     hip_lib.element_types()[self.dtype], lib.stream(x))
+        return x
+
+
+def empty_checkpoint8(x):
+    """Checkpoint8 of x's type for rows x's leading dimensions, not yet written."""
+    rows, channels = x.shape[:-1].numel(), x.shape[-1]
+    blocks = -(-channels // BLOCK)
+    return Checkpoint8(torch.empty(rows, BLOCK * blocks, dtype=torch.int8, device=x.device),
+                       torch.empty(blocks, rows, dtype=torch.uint8, device=x.device), channels, x.dtype, x.shape)
+
+
+def checkpoint8(x):
+    """The 8-bit checkpoint of x [..., channels] (no gradient flows through it).  Blocks run along the last dimension: hand a
+    channels-last image over as ``x.movedim(1, -1)``."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise hip_lib.SaeError("checkpoint8: at least one value in the last dimension, got shape %s" % (tuple(x.shape),))
+    lib = hip_lib.get()
+    x = hip_lib.dense(x.detach())
+    lib.check_channels_last(x)
+    kept = empty_checkpoint8(x)
+    with lib.device_of(x):
+        lib.call("checkpoint8_pack", x.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), kept.rows, kept.channels,
+                 hip_lib.element_types()[x.dtype], lib.stream(x))
+    return kept
+
+
+def linear_weight_grad8(gy, kept, bias=True, alpha=1.0):
+    """(gw [out, channels], gb [out] or None) of ``alpha * x @ weight.T + bias`` from gy [..., out] and the Checkpoint8 of x:
+    gw = alpha * gy^T x8, gb = the sum of gy's rows.  In gy's type, which has to be the checkpoint's; the products are exact and
+    added in fp32 (f32: gy in three bf16 pieces, which hold all of its 24 bits)."""
+    lib = hip_lib.get()
+    if gy.dim() < 1 or gy.shape[-1] < 1 or gy.shape[:-1].numel() != kept.rows:
+        raise hip_lib.SaeError("linear_weight_grad8: gy %s does not have the checkpoint's %d rows" % (tuple(gy.shape), kept.rows))
+    if gy.dtype != kept.dtype or gy.device != kept.codes.device:
+        raise hip_lib.SaeError("linear_weight_grad8: gy is %s on %s, the checkpoint %s on %s"
+                               % (gy.dtype, gy.device, kept.dtype, kept.codes.device))
+    gy = hip_lib.dense(gy.detach())
+    lib.check_channels_last(gy)
+    out, c = gy.shape[-1], kept.channels
+    gw = torch.empty(out, c, dtype=gy.dtype, device=gy.device)
+    gb = torch.empty(out, dtype=gy.dtype, device=gy.device) if bias else None
+    n_ws = lib.query("linear_wgrad8_workspace", kept.rows, out, c)
+    ws = torch.empty(max(n_ws, 1), dtype=torch.float32, device=gy.device)
+    with lib.device_of(gy):
+        lib.call("linear_wgrad8", gy.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), gw.data_ptr(), hip_lib.ptr(gb),
+                 kept.rows, out, c, float(alpha), hip_lib.element_types()[gy.dtype], ws.data_ptr(), n_ws, lib.stream(gy))
+    return gw, gb
+
+
+class Linear8(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, alpha, train):
+        y = _gemm(x, weight, bias, False, True, alpha)
+        if train:
+            kept = checkpoint8(x) if weight.requires_grad else None
+            ctx.save_for_backward(weight, *((kept.codes, kept.scales) if kept is not None else ()))
+            ctx.cfg = (alpha, bias is not None)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        weight, *kept = ctx.saved_tensors
+        alpha, has_bias = ctx.cfg
+        gy = hip_lib.dense(gy)
+        gx = gw = gb = None
+        if ctx.needs_input_grad[0]:
+            gx = _gemm(gy, weight, None, False, False, alpha)
+        if ctx.needs_input_grad[1] and _Flags.weight_grads:
+            gw, gb = linear_weight_grad8(gy, Checkpoint8(*kept, weight.shape[1], torch.float32), has_bias, alpha)
+        if ctx.needs_input_grad[2] and gb is None:
+            gb = gy.sum(0)
+        return gx, gw, gb, None, None
+
+
+def linear8(input, weight, bias=None, alpha=1.0):
+    """``linear`` (alpha * input @ weight^T + bias, float32) whose backward takes the weight gradient from the 8-bit checkpoint of
+    the input; y and the input gradient are ``linear``'s.  Differentiable once."""
+    lead = input.shape[:-1]
+    x2 = input.reshape(-1, input.shape[-1])
+    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, bias))
+    return Linear8.apply(x2, weight, bias, alpha, train).view(*lead, weight.shape[0])
+
+
+def _own_or_view_of_leaf(t):
+    base = t if t._base is None else t._base
+    return base.is_leaf and base.requires_grad
+
+
+class _Kept:
+    """One packed activation: the checkpoint of its memory in order, and the strides it had."""
+    __slots__ = ("kept", "size", "stride")
+
+
+def _pack(t, least):
+    if t.dtype not in hip_lib.element_types() or t.numel() < least or _own_or_view_of_leaf(t):
+        return t
+    order = sorted(range(t.dim()), key=lambda d: (-t.stride(d), d))
+    flat = t.detach().permute(order)
+    if not flat.is_contiguous():          # expanded, overlapping or with gaps: as it is
+        return t
+    k = _Kept()
+    k.size, k.stride = t.size(), t.stride()
+    n = t.numel()
+    # rows of 4096 values where the memory divides into them: whole blocks either way, the last one alone may be short
+    k.kept = checkpoint8(flat.reshape(-1, 4096) if n % 4096 == 0 else flat.reshape(1, n))
+    return k
+
+
+def _unpack(k):
+    if not isinstance(k, _Kept):
+        return k
+    return k.kept.dequantize().view(-1).as_strided(k.size, k.stride)
+
+
+@contextlib.contextmanager
+def activation_checkpoints8(least=65536, enabled=True):
+    """Every autograd node built inside keeps the activations it saves (float32, bfloat16, float16; at least ``least`` values) as
+    8-bit checkpoints and gets them back when its backward runs, wherever that is.  Leaves that require a gradient (parameters,
+    and what is a view of one) and small tensors are kept as they are.  Forward values do not change; gradients are those at the
+    values that the checkpoints stand for."""
+    if not enabled:
+        yield
+        return
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: _pack(t, least), _unpack):
+        yield

@@ -34,13 +34,28 @@ def needs_build():
 def build(force=False):
     if not force and not needs_build():
         return OUT
-    cmd = [host_clang(), "-x", "c++", "-std=c++17", "-O2", "-fPIC", "-shared", "-nogpulib", "-Wno-unused-value", "-Wno-psabi",
-           "-DSAE_TUNING", "-I", HERE, "-I", os.path.join(ROOT, "include"), "-I", CSRC]
-    for s in sources():
-        cmd += [s]
-    cmd += ["-o", OUT]
-    # every source must be treated as C++ (the .hip suffix would select the HIP language)
-    subprocess.check_call(cmd)
+    # one object per source, side by side (git-ignored; only the linked library is loaded); .hip would select the HIP language
+    from concurrent.futures import ThreadPoolExecutor
+    objdir = os.path.join(HERE, "build")
+    os.makedirs(objdir, exist_ok=True)
+    flags = ["-x", "c++", "-std=c++17", "-O2", "-fPIC", "-nogpulib", "-Wno-unused-value", "-Wno-psabi", "-DSAE_TUNING", "-I", HERE,
+             "-I", os.path.join(ROOT, "include"), "-I", CSRC]
+    shared = [os.path.join(CSRC, "sae_common.h"), os.path.join(ROOT, "include", "sae_hip.h"),
+              os.path.join(HERE, "hip", "hip_runtime.h")]
+    if ROOT not in sys.path:
+        sys.path.insert(0, ROOT)
+    from swapping_autoencoder_pytorch_amd.csrc.build import _included as included
+
+    def one(src):
+        obj = os.path.join(objdir, os.path.basename(src) + ".o")
+        deps = [src] + shared + included(src)
+        if force or not os.path.exists(obj) or any(os.path.getmtime(d) > os.path.getmtime(obj) for d in deps):
+            subprocess.check_call([host_clang()] + flags + ["-c", src, "-o", obj])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=min(6, os.cpu_count() or 1)) as ex:
+        objs = list(ex.map(one, sources()))
+    subprocess.check_call([host_clang(), "-shared", "-fPIC"] + objs + ["-o", OUT])
     return OUT
 
 

@@ -47,6 +47,7 @@ struct dim3 {
 };
 struct float2 { float x, y; };
 struct float4 { float x, y, z, w; };
+struct double2 { double x, y; };
 struct int2 { int x, y; };
 struct int4 { int x, y, z, w; };
 static inline float2 make_float2(float x, float y) { return float2{x, y}; }
@@ -307,6 +308,27 @@ inline f32x16 mfma_32x32x16bf16(bf16x8 a, bf16x8 b, f32x16 c, int, int, int) {
     return c;
 }
 
+// v_mfma_f32_32x32x16_f16: the lane layout of the bf16 form
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+inline f32x16 mfma_32x32x16f16(f16x8 a, f16x8 b, f32x16 c, int, int, int) {
+    WaveState& W = my_wave();
+    const int l = lane_id();
+    const int slot = W.gen & 1;
+    std::memcpy(W.ha[slot][l], &a, 16);
+    std::memcpy(W.hb[slot][l], &b, 16);
+    wave_rendezvous(W);
+    auto value = [](uint16_t h) { _Float16 f; std::memcpy(&f, &h, 2); return (double)(float)f; };
+    const int col = l & 31;
+    for (int r = 0; r < 16; ++r) {
+        const int row = (r & 3) + 8 * (r >> 2) + 4 * (l >> 5);
+        double acc = c[r];
+        for (int k = 0; k < 16; ++k)
+            acc += value(W.ha[slot][(k >> 3) * 32 + row][k & 7]) * value(W.hb[slot][(k >> 3) * 32 + col][k & 7]);
+        c[r] = (float)acc;
+    }
+    return c;
+}
+
 template <typename T>
 inline T exchange(T v, int src_lane) {
     static_assert(sizeof(T) <= 8, "hipemu exchange: type too wide");
@@ -337,6 +359,7 @@ static inline void __syncthreads() { hipemu::block_barrier(); }
 #define __builtin_amdgcn_mfma_f32_32x32x2f32 hipemu::mfma_32x32x2f32
 #define __builtin_amdgcn_mfma_f32_16x16x4f32 hipemu::mfma_16x16x4f32
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16 hipemu::mfma_32x32x16bf16
+#define __builtin_amdgcn_mfma_f32_32x32x16_f16 hipemu::mfma_32x32x16f16
 // LDS-DMA (global_load_lds_*): lane l of the wave writes `size` bytes at (wave-uniform LDS base) + size * l.
 // The copy is performed at once; the real instruction is asynchronous (ordered by vmcnt + a barrier), which
 // a correct program cannot observe.
