@@ -1655,8 +1655,8 @@ int oracle_group_norm_act_bwd(const void* gy, const void* x, const int8_t* codes
     return SAE_OK;
 }
 
-int64_t oracle_linear_wgrad8_workspace(int64_t rows, int64_t out, int64_t c) {
-    (void)rows; (void)out; (void)c;
+int64_t oracle_linear_wgrad8_workspace(int64_t rows, int64_t out, int64_t c, int32_t dtype) {
+    (void)rows; (void)out; (void)c; (void)dtype;
     return 4;
 }
 

@@ -6,15 +6,21 @@
 //     x8 = q * 2^k has 8 significant bits at most: a bf16 (and, with k >= -24, an f16) value exactly
 //     gy in bf16 / f16 is taken as it is
 //     gy in f32 is cut into three bf16 pieces of 8 bits each, high + middle + low = gy exactly, and takes three products
-// v_mfma_f32_32x32x16 at 3 products is ~5 times v_mfma_f32_32x32x2_f32's rate: keeping x in 8 bits makes the f32 weight gradient
-// faster than the exact f32 product of the full-width tensors, not only smaller.
+// v_mfma_f32_32x32x16 at 3 products has five times the rate of v_mfma_f32_32x32x2_f32: keeping x in 8 bits makes the f32 weight
+// gradient faster than the exact f32 product of the full-width tensors, not only smaller.
 //
-// Tile: BM channels of gy x 128 channels of x, 32 rows at a time.  The sum runs over ROWS, the slow axis of both tensors, while a
-// matrix-core operand wants 8 rows of one channel next to each other: a thread loads 4 channels of 4 rows (16 bytes a row of f32
-// gy, 4 bytes a row of codes), and writes for each of its 4 channels the 4 rows packed to 8 bytes.  LDS holds 16-byte cells
-// [k octet][position], where channel 4 j + m of a group of 128 sits at position 32 m + j: lanes that stage neighbouring quads
-// write neighbouring cells, an operand is one 16-byte read with neighbouring lanes on neighbouring cells, and a lane ends up with
-// the 4 neighbouring output channels 4 j ... 4 j + 3 in its 4 accumulators -- whole 16-byte stores, no shuffle.
+// Tile: BM channels of gy x 128 channels of x, 32 rows (f32) or 64 at a time, four waves.  The sum runs over ROWS, the slow axis of
+// both tensors, while a matrix-core operand wants 8 rows of one channel next to each other: a thread loads 4 channels of 4 rows (16
+// bytes a row of f32 gy, 4 bytes a row of codes), and writes for each of its 4 channels the 4 rows packed to 8 bytes.  LDS holds
+// 16-byte cells [k octet][position], where channel 4 j + m of a group of 128 sits at position 32 m + j: lanes that stage neighbouring
+// quads write neighbouring cells, an operand is one 16-byte read with neighbouring lanes on neighbouring cells (no bank conflict, by
+// the counters), and a lane ends up with the 4 neighbouring output channels 4 j ... 4 j + 3 in its 4 accumulators -- whole 16-byte
+// stores, no shuffle.
+//
+// What bounds it: a wave issues in order, so everything a step needs beside its products -- cutting gy, decoding codes, LDS writes,
+// the loads two steps ahead -- is dealt out between them (`multiply`).  Measured on f32 16384 x 1024 x 2048: 340 us with one set of
+// cells and a burst of each; 229 us with two groups of four waves that stage and multiply in turn (their loads, one step ahead, are
+// waited for); 206 us in this form, of which the products alone take 140.  bf16 65536 x 512 x 512: 140 -> 77 us.
 //
 // Few tiles: the rows are cut into slices, one work-group each, whose fp32 tiles a second kernel adds in order.
 #include "elem8.inc"
@@ -23,8 +29,6 @@ namespace sae {
 namespace {
 
 constexpr int kBN = 128;       // channels of x of a tile
-constexpr int kRows = 32;      // rows of a step
-constexpr int kOct = kRows / 8;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -37,11 +41,36 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// two values that are exact in 16 bits, as a word (low half: the first)
+// the low or high halves of two words, as a word (low half: a's)
+template <bool HIGH>
+__device__ __forceinline__ unsigned halves(unsigned a, unsigned b) {
+#ifdef HIPEMU
+    return HIGH ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | (b << 16);
+#else
+    return __builtin_amdgcn_perm(b, a, HIGH ? 0x07060302u : 0x05040100u);
+#endif
+}
+// two values that are exact in 16 bits, as a word
 template <int DT>
 __device__ __forceinline__ unsigned pack_exact(float a, float b) {
     if constexpr (DT == SAE_F16) return (unsigned)narrow<DT>(a) | ((unsigned)narrow<DT>(b) << 16);
-    else return (f_bits(a) >> 16) | (f_bits(b) & 0xffff0000u);
+    else return halves<true>(f_bits(a), f_bits(b));
+}
+
+// sum + the two 16-bit values of a word, widened
+template <int DT>
+__device__ __forceinline__ float add_pair(float sum, unsigned w) {
+#ifdef HIPEMU
+    return sum + (widen<DT>((uint16_t)(w & 0xffffu)) + widen<DT>((uint16_t)(w >> 16)));
+#else
+    if constexpr (DT == SAE_BF16) {
+        typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, w), __builtin_bit_cast(v2, 0x3f803f80u), sum, false);
+    } else {
+        typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, w), __builtin_bit_cast(v2, 0x3c003c00u), sum, false);
+    }
+#endif
 }
 
 struct WgShape {
@@ -51,217 +80,376 @@ struct WgShape {
     int64_t slice_rows;
 };
 
+// A slice's rows of a tensor behind a range-checked descriptor: a row behind the last reads as zero, without a mask
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+
 // A thread's 4 rows x 4 channels of gy, as loaded
 template <int DT, bool VEC>
 struct GyQuad {
+    using T = typename Elem<DT>::T;
     float f[4][4];     // f32
     u32x2 h[4];        // 16-bit types: 4 channels of a row
-    __device__ __forceinline__ void load(const typename Elem<DT>::T* __restrict__ gy, int64_t r0, int64_t r_end, int o, int out) {
+    // row i: r0 + mine + i of a slice of `rows` (r0 the same in a wave, mine not), channels o ... o + 3 of it.
+    // VEC: the quad is there or not (out % 4 == 0); mine and o are in the lane's offset `at`, r0 in the scalar one, which stays
+    // within the descriptor
+    __device__ __forceinline__ void load(int i, __amdgpu_buffer_rsrc_t all, unsigned at, const T* __restrict__ gy, int r0, int mine,
+                                         int rows, int o, int out) {
+        if constexpr (VEC) {
+            const unsigned from = (unsigned)(r0 + i < rows ? r0 + i : rows) * (unsigned)out * (unsigned)sizeof(T);
+            if constexpr (DT == SAE_F32) {
+                const u32x4 q = __builtin_amdgcn_raw_buffer_load_b128(all, at, from, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool on = r0 + i < r_end;
-            const typename Elem<DT>::T* p = gy + (r0 + i) * (int64_t)out + o;
-            if constexpr (VEC) {                                   // out % 4 == 0: the quad is there or not
-                const bool in = on && o < out;
-                if constexpr (DT == SAE_F32) {
-                    f32x4 q = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (in) q = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) f[i][j] = q[j];
-                } else {
-                    h[i] = u32x2{0u, 0u};
-                    if (in) h[i] = *reinterpret_cast<const u32x2*>(p);
-                }
-            } else if constexpr (DT == SAE_F32) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f[i][j] = on && o + j < out ? p[j] : 0.0f;
+                for (int j = 0; j < 4; ++j) f[i][j] = bits_f(q[j]);
             } else {
-                unsigned v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = on && o + j < out ? p[j] : 0u;
-                h[i] = u32x2{v[0] | (v[1] << 16), v[2] | (v[3] << 16)};
+                h[i] = __builtin_amdgcn_raw_buffer_load_b64(all, at, from, 0);
             }
+        } else {
+            const bool on = r0 + mine + i < rows;
+            const T* p = gy + (int64_t)(r0 + mine + i) * out + o;
+            unsigned v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const T e = on && o + j < out ? p[j] : (T)0;
+                if constexpr (DT == SAE_F32) f[i][j] = e;
+                else v[j] = e;
+            }
+            if constexpr (DT != SAE_F32) h[i] = u32x2{v[0] | (v[1] << 16), v[2] | (v[3] << 16)};
         }
     }
-    __device__ __forceinline__ unsigned half(int i, int j) const { return (h[i][j >> 1] >> (16 * (j & 1))) & 0xffffu; }
+    // channel j of rows i and i + 1, as a word (16-bit types)
+    __device__ __forceinline__ unsigned pair(int i, int j) const {
+        return j & 1 ? halves<true>(h[i][j >> 1], h[i + 1][j >> 1]) : halves<false>(h[i][j >> 1], h[i + 1][j >> 1]);
+    }
     __device__ __forceinline__ float value(int i, int j) const {
         if constexpr (DT == SAE_F32) return f[i][j];
-        else return widen<DT>((uint16_t)half(i, j));
+        else return widen<DT>((uint16_t)(h[i][j >> 1] >> (16 * (j & 1))));
     }
 };
 
-// high part of v in 8 bits (cut, not rounded: the rest is exact); an infinity or NaN has no rest
-__device__ __forceinline__ float cut8(float v) { return bits_f(f_bits(v) & 0xffff0000u); }
+// the rest of v behind its high 8 bits (cut, not rounded: the rest is exact); ODD: an infinity or NaN has none
+template <bool ODD>
+__device__ __forceinline__ float rest8(float v) {
+    const float rest = v - bits_f(f_bits(v) & 0xffff0000u);
+    if constexpr (ODD) return (f_bits(v) & 0x7f800000u) == 0x7f800000u ? 0.0f : rest;
+    else return rest;
+}
 
-template <int DT, int BM, bool VEC>
-__global__ __launch_bounds__(kBlock) void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy,
-                                                               const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                               float* __restrict__ part, float* __restrict__ part_b, const WgShape p) {
-    constexpr int PL = DT == SAE_F32 ? 3 : 1;                     // pieces of gy
-    constexpr int NQ = BM / 4 * (kRows / 4) / kBlock > 0 ? BM / 4 * (kRows / 4) / kBlock : 1;   // gy quads of a thread
-    constexpr int MT = BM / 64;                                   // 32-channel tiles of gy in a wave: 64 x 128 (BM 256) ...
-    constexpr int WN = BM >= 128 ? 4 : 2;                         // ... 32 x 128 (128), 32 x 64 (64)
-    static_assert(BM == 64 || BM == 128 || BM == 256, "tile");
-    constexpr int WM = BM == 256 ? 2 : 1;
-    (void)MT;
-    __shared__ u32x4 As[PL][kOct][BM];
-    __shared__ u32x4 Bs[kOct][kBN];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, l31 = lane & 31, half = lane >> 5;
-    // slices of the same rows on one XCD (work-groups go round the eight of them): its L2 serves the tiles' shared reads
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int slice = blockIdx.x / tiles, tile = blockIdx.x - slice * tiles;
+template <int DT, int BM>
+struct WgTile {
+    static constexpr int PL = DT == SAE_F32 ? 3 : 1;              // pieces of gy
+    static constexpr int KR = DT == SAE_F32 ? 32 : 64;            // rows of a step: 2 x 56 / 2 x 48 KB of LDS at BM = 256
+    static constexpr int OCT = KR / 8;
+    static constexpr int AQ = BM / 4 * (KR / 4);                  // gy quads of a step
+    static constexpr int NA = AQ / kBlock > 0 ? AQ / kBlock : 1;  // of a thread
+    static constexpr int AR = kBlock / (BM / 4);                  // row quads that the threads cover at once
+    static constexpr int NB = kBN / 4 * (KR / 4) / kBlock;        // codes quads of a thread
+    static constexpr int WM = BM == 256 ? 2 : 1;                  // 32-channel tiles of a wave: 64 x 128 (BM 256),
+    static constexpr int WN = BM == 64 ? 2 : 4;                   // 32 x 128 (128), 32 x 64 (64)
+    static constexpr int CELLS = OCT * (PL * BM + kBN);           // 16-byte cells of a step
+    // position of channel 4 q + j: groups of 128 channels, 32 j + q inside (BM = 64: 16 j + q)
+    static __device__ __forceinline__ int place(int q, int j) { return BM == 64 ? 16 * j + q : (q >> 5) * 128 + 32 * j + (q & 31); }
+    static __device__ __forceinline__ int channel(int at) {
+        return BM == 64 ? 4 * (at & 15) + (at >> 4) : (at >> 7) * 128 + 4 * (at & 31) + ((at >> 5) & 3);
+    }
+};
+
+template <int DT, int BM, bool VEC, bool WHOLE>
+__global__ __launch_bounds__(kBlock, BM == 256 ? 1 : 2)
+void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int8_t* __restrict__ codes,
+                          const uint8_t* __restrict__ scales, float* __restrict__ part, float* __restrict__ part_b,
+                          typename Elem<DT>::T* __restrict__ gw, typename Elem<DT>::T* __restrict__ gb, float alpha, const WgShape p) {
+    using W = WgTile<DT, BM>;
+    using T = typename Elem<DT>::T;
+    constexpr int PL = W::PL, KR = W::KR, OCT = W::OCT, NA = W::NA, NB = W::NB, WM = W::WM, WN = W::WN, AR = W::AR;
+    __shared__ u32x4 cells[2][W::CELLS];                          // of a step: gy [PL][OCT][BM], codes [OCT][kBN]
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Work-groups go round the eight XCDs.  Each XCD takes a run of neighbouring (slice, tile row, tile column): whole slices where
+    // there are eight or more, else tile rows of one, so that its L2 reads a tile of gy once for all the columns beside it.
+    const int tiles = p.tiles_m * p.tiles_n, all = (int)gridDim.x, xcd = blockIdx.x & 7;
+    const int run = xcd * (all >> 3) + (xcd < (all & 7) ? xcd : (all & 7)) + (int)(blockIdx.x >> 3);
+    const int slice = run / tiles, tile = run - slice * tiles;
     const int tn = tile % p.tiles_n, tm = tile / p.tiles_n;
     const int o0 = tm * BM, i0 = tn * kBN;
     const int64_t r_begin = slice * p.slice_rows;
     const int64_t r_end = r_begin + p.slice_rows < p.rows ? r_begin + p.slice_rows : p.rows;
-
-    f32x16 acc[WM][WN];
-#pragma unroll
-    for (int m = 0; m < WM; ++m)
-#pragma unroll
-        for (int n = 0; n < WN; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[m][n][r] = 0.0f;
-    float sum[NQ][4];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum[q][j] = 0.0f;
-
-    const int bq = tid & 31, br = tid >> 5;                       // codes: channel quad, row quad
-    const int bc = i0 + 4 * bq;
-    const bool b_in = bc < p.blocks * kBlk8;
-    const int8_t* const bsrc = codes + (b_in ? bc : 0);
-    const uint8_t* const ssrc = scales + (int64_t)(b_in ? bc / kBlk8 : 0) * p.rows;
+    const int rows = (int)(r_end - r_begin), steps = (rows + KR - 1) / KR;
+    const int last = (int)(p.rows - r_begin) - 4;
     const int64_t ld = (int64_t)p.blocks * kBlk8;
 
-    for (int64_t r0 = r_begin; r0 < r_end; r0 += kRows) {
-        GyQuad<DT, VEC> g[NQ];
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            const int e = tid + q * kBlock, oq = e % (BM / 4), rq = e / (BM / 4);
-            g[q].load(gy, r0 + 4 * rq, rq < kRows / 4 ? r_end : r_begin, o0 + 4 * oq, p.out);
+    f32x16 acc[WM][WN];
+    float sum[4];                                                 // gb: the thread's channels are the same in every step
+
+    // what a step's loads bring a thread; two steps are under way
+    struct Load {
+        GyQuad<DT, VEC> g[NA];
+        unsigned cw[NB][4], ce[NB];
+    };
+    Load load[2];
+    // neighbouring lanes take the two row quads of a cell: their 8-byte writes fill whole cells, without a bank conflict
+    const int oq = (tid >> 1) % (BM / 4), ar = (tid & 1) + 2 * (tid / (BM / 2));   // gy: channel quad, row quad (of every AR)
+    const int bq = (tid >> 1) & 31, br = (tid & 1) + 2 * (tid >> 6);               // codes: channel quad, row quad (of every 8)
+    const bool a_in = W::AQ >= kBlock || ar < KR / 4, b_in = i0 + 4 * bq < ld;
+    const T* const gsrc = gy + r_begin * p.out;
+    const __amdgpu_buffer_rsrc_t grows = rows_of(gsrc, (int64_t)rows * p.out * (int64_t)sizeof(T));
+    const __amdgpu_buffer_rsrc_t crows = rows_of(codes + r_begin * ld, rows * ld);
+    const uint8_t* const ssrc = scales + (int64_t)(b_in ? (i0 + 4 * bq) / kBlk8 : 0) * p.rows + r_begin;
+    const unsigned nowhere = 0xfffffff0u;                         // behind every descriptor
+    const unsigned gat = a_in && o0 + 4 * oq < p.out
+                             ? ((unsigned)(4 * ar) * (unsigned)p.out + (unsigned)(o0 + 4 * oq)) * (unsigned)sizeof(T) : nowhere;
+    const unsigned cat = b_in ? (unsigned)(4 * br) * (unsigned)ld + (unsigned)(i0 + 4 * bq) : nowhere;
+
+    auto fetch_gy = [&](Load& to, int step, int n) {              // n < 4 NA: one row of a quad
+        to.g[n >> 2].load(n & 3, grows, gat, gsrc, step * KR + 4 * AR * (n >> 2), 4 * ar, a_in ? rows : 0, o0 + 4 * oq, p.out);
+    };
+    auto fetch_codes = [&](Load& to, int step, int n) {           // n < 5 NB: four rows of a quad, and their exponents
+        const int q = n / 5, i = n % 5;
+        if (i < 4) {
+            const int from = step * KR + 32 * q + i;
+            to.cw[q][i] = __builtin_amdgcn_raw_buffer_load_b32(crows, cat, (unsigned)(from < rows ? from : rows) * (unsigned)ld, 0);
+            return;
         }
-        unsigned cw[4], ce[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t r = r0 + 4 * br + i;
-            const bool on = b_in && r < r_end;
-            cw[i] = on ? *reinterpret_cast<const unsigned*>(bsrc + r * ld) : 0u;
-            ce[i] = on ? ssrc[r] : 0u;
+        const int r = step * KR + 4 * (br + 8 * q);
+        if (p.rows >= 4) {                                        // a word that ends at the block's last row at most
+            __builtin_memcpy(&to.ce[q], ssrc + (r < last ? r : last), 4);
+        } else {
+            to.ce[q] = 0;
+            for (int i = 0; i < rows; ++i) to.ce[q] |= (unsigned)ssrc[i] << (8 * i);
+            to.ce[q] <<= 8 * -last;
         }
-        __syncthreads();
+    };
+    auto fetch = [&](Load& to, int step, bool all_of_it) {
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            const int e = tid + q * kBlock, oq = e % (BM / 4), rq = e / (BM / 4);
-            if (rq < kRows / 4) {
+        for (int n = 0; n < 4 * NA; ++n) fetch_gy(to, step, n);
+        if (all_of_it)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    // channel 4 oq + j: group of 128, position 32 j + (oq & 31) in it (BM = 64: 16 j + oq)
-                    const int pos = BM == 64 ? 16 * j + oq : (oq >> 5) * 128 + 32 * j + (oq & 31);
-                    if constexpr (DT == SAE_F32) {
-                        float v[4];
+            for (int n = 0; n < 5 * NB; ++n) fetch_codes(to, step, n);
+    };
+    auto put = [&](u32x4* cell, int rq, unsigned lo, unsigned hi) { *(reinterpret_cast<u32x2*>(cell) + (rq & 1)) = u32x2{lo, hi}; };
+    // One channel of a quad: of gy (n < 4 NA) or of the codes.  ODD: with infinities and NaN among the values (f32)
+    constexpr int PIECES = 4 * (NA + NB);
+    auto stage = [&](const Load& from, int step, u32x4* to, int n, auto odd) {
+        if (n < 4 * NA) {
+            const int q = n >> 2, j = n & 3, rq = ar + AR * q;
+            u32x4* const row = to + (rq >> 1) * BM + W::place(oq, j);
+            if constexpr (DT == SAE_F32) {
+                float v[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = g[q].f[i][j];
-#pragma unroll
-                        for (int s = 0; s < 3; ++s) {
-                            u32x2* cell = reinterpret_cast<u32x2*>(&As[s][rq >> 1][pos]) + (rq & 1);
-                            *cell = u32x2{pack_exact<DT>(v[0], v[1]), pack_exact<DT>(v[2], v[3])};
-                            if (s < 2)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) v[i] = (f_bits(v[i]) & 0x7f800000u) == 0x7f800000u ? 0.0f : v[i] - cut8(v[i]);
-                        }
-                    } else {
-                        u32x2* cell = reinterpret_cast<u32x2*>(&As[0][rq >> 1][pos]) + (rq & 1);
-                        *cell = u32x2{g[q].half(0, j) | (g[q].half(1, j) << 16), g[q].half(2, j) | (g[q].half(3, j) << 16)};
-                    }
-                    if (tn == 0)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sum[q][j] += g[q].value(i, j);
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = from.g[q].f[i][j];
+                    sum[j] += v[i];
+                    if (odd.value && v[i] != v[i]) v[i] = bits_f(0x7fc00000u);       // (a NaN of low bits alone is cut to infinity)
                 }
-            }
-        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+                for (int s = 0; s < 3; ++s) {
+                    if (W::AQ >= kBlock || rq < KR / 4)
+                        put(row + s * OCT * BM, rq, pack_exact<DT>(v[0], v[1]), pack_exact<DT>(v[2], v[3]));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = rest8<odd.value>(v[i]);
+                }
+            } else {
+                const unsigned lo = from.g[q].pair(0, j), hi = from.g[q].pair(2, j);
+                sum[j] = add_pair<DT>(add_pair<DT>(sum[j], lo), hi);
+                if (W::AQ >= kBlock || rq < KR / 4) put(row, rq, lo, hi);
+            }
+        } else {
+            const int q = (n >> 2) - NA, j = n & 3, rq = br + 8 * q, r = step * KR + 4 * rq;
+            const int by = r < last ? 0 : r - last, have = rows - r;    // the word shifted, and cut to the slice's rows
+            const unsigned e = have <= 0 ? 0u : (from.ce[q] >> (8 * by)) & (have >= 4 ? 0xffffffffu : (1u << (8 * have)) - 1u);
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(cw[i] >> (8 * j)) * block8_step(ce[i]);
-            u32x2* cell = reinterpret_cast<u32x2*>(&Bs[br >> 1][32 * j + bq]) + (br & 1);
-            *cell = u32x2{pack_exact<DT>(v[0], v[1]), pack_exact<DT>(v[2], v[3])};
+            for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(from.cw[q][i] >> (8 * j)) * block8_step((e >> (8 * i)) & 0xffu);
+            put(to + PL * OCT * BM + (rq >> 1) * kBN + 32 * j + bq, rq, pack_exact<DT>(v[0], v[1]), pack_exact<DT>(v[2], v[3]));
         }
-        __syncthreads();
+    };
+    // The products of a step out of `from`, and between them, a share behind each PL-th part, whatever `beside` does: matrix cores
+    // and vector units work at the same time, from one wave.  Operands are read one part ahead.
+    constexpr int PARTS = KR / 16 * PL;
+    auto multiply = [&](const u32x4* from, auto beside) {
+        u32x4 bf[2][WN], af[2][WM];
+        auto read = [&](int part) {
+            const int s = part / PL, k = part % PL;
+            if (k == 0)
 #pragma unroll
-        for (int s = 0; s < kRows / 16; ++s) {
-            u32x4 bf[WN], af[WM][PL];
+                for (int n = 0; n < WN; ++n)
+                    bf[s & 1][n] = from[PL * OCT * BM + (2 * s + half) * kBN + 32 * (BM == 64 ? 2 * (wid & 1) + n : n) + l31];
 #pragma unroll
-            for (int n = 0; n < WN; ++n) bf[n] = Bs[2 * s + half][32 * (BM == 64 ? 2 * (wid & 1) + n : n) + l31];
+            for (int m = 0; m < WM; ++m)
+                af[part & 1][m] = from[(k * OCT + 2 * s + half) * BM + 32 * (BM == 64 ? wid >> 1 : wid * WM + m) + l31];
+        };
+        read(0);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+            if (part + 1 < PARTS) read(part + 1);
 #pragma unroll
             for (int m = 0; m < WM; ++m)
 #pragma unroll
-                for (int k = 0; k < PL; ++k) af[m][k] = As[k][2 * s + half][32 * (BM == 64 ? wid >> 1 : wid * WM + m) + l31];
+                for (int n = 0; n < WN; ++n) acc[m][n] = mma<DT>(af[part & 1][m], bf[(part / PL) & 1][n], acc[m][n]);
+            beside(part);
+            // operand reads, then a product, a share of the vector work and of the memory instructions in turn: a wave issues in
+            // order, and loads that come in a burst wait for the CU's one address unit with every product behind them
+            __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
 #pragma unroll
-            for (int k = 0; k < PL; ++k)
+            for (int i = 0; i < WM * WN; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto clear = [&]() {
 #pragma unroll
-                for (int m = 0; m < WM; ++m)
+        for (int m = 0; m < WM; ++m)
 #pragma unroll
-                    for (int n = 0; n < WN; ++n) acc[m][n] = mma<DT>(af[m][k], bf[n], acc[m][n]);
+            for (int n = 0; n < WN; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[m][n][r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = 0.0f;
+    };
+
+    clear();
+    fetch(load[0], 0, true);
+    fetch(load[1], 1, true);
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n) stage(load[0], 0, cells[0], n, BoolTag<false>());
+    fetch(load[0], 2, false);
+    __syncthreads();
+    // Step t: products of cells[t & 1]; what was loaded of step t + 1 goes to the other cells, and step t + 3 of gy is asked for into
+    // the registers that this frees, step t + 2 of the codes into those freed in the step before.  (Steps behind the last are zeros.)
+    constexpr int LOADS = 5 * NB + 4 * NA;
+    auto turn = [&](int step, Load& next, Load& before, const u32x4* from, u32x4* to) {
+        multiply(from, [&](int part) {
+#pragma unroll
+            for (int n = PIECES * part / PARTS; n < PIECES * (part + 1) / PARTS; ++n) stage(next, step + 1, to, n, BoolTag<false>());
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n) {
+                if (n * PARTS / LOADS != part) continue;
+                if (n < 5 * NB) {
+                    fetch_codes(before, step + 2, n);
+                } else {
+                    const int m = n - 5 * NB;                     // (its quad is staged by then)
+                    static_assert(5 * NB * PARTS / LOADS >= 3 * PARTS / PIECES && (LOADS - 4) * PARTS / LOADS >= (4 * NA - 1) * PARTS / PIECES, "order");
+                    fetch_gy(next, step + 3, m);
+                }
+            }
+        });
+        __syncthreads();
+    };
+    for (int step = 0; step < steps; step += 2) {
+        turn(step, load[1], load[0], cells[0], cells[1]);
+        if (step + 1 < steps) turn(step + 1, load[0], load[1], cells[1], cells[0]);
+    }
+    if constexpr (DT == SAE_F32) {
+        // An infinity or NaN in gy makes the rest behind its high piece a NaN, and with it the whole row of the tile: such a tile is
+        // computed again with the pieces of these values set right.
+        float zero = 0.0f;
+#pragma unroll
+        for (int m = 0; m < WM; ++m)
+#pragma unroll
+            for (int n = 0; n < WN; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) zero = fmaf(acc[m][n][r], 0.0f, zero);
+        int* const flag = reinterpret_cast<int*>(&cells[0][0]);
+        if (tid == 0) *flag = 0;
+        __syncthreads();
+        if (zero != 0.0f || zero != zero) *flag = 1;
+        __syncthreads();
+        const bool again = *flag != 0;
+        __syncthreads();
+        if (again) {
+            clear();
+            for (int step = 0; step < steps; ++step) {
+                fetch(load[0], step, true);
+#pragma unroll
+                for (int n = 0; n < PIECES; ++n) stage(load[0], step, cells[0], n, BoolTag<true>());
+                __syncthreads();
+                multiply(cells[0], [](int) {});
+                __syncthreads();
+            }
         }
     }
-    // accumulator register r of the lane: tile row (r & 3) + 8 (r >> 2) + 4 half, tile column l31
-    float* const dst = part + (int64_t)slice * p.out * ld;
+
+    // register r of the lane: tile row (r & 3) + 8 (r >> 2) + 4 half, tile column l31
 #pragma unroll
     for (int m = 0; m < WM; ++m) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int at = 32 * (BM == 64 ? wid >> 1 : wid * WM + m) + (r & 3) + 8 * (r >> 2) + 4 * half;    // position of the row
-            const int o = o0 + (BM == 64 ? 4 * (at & 15) + (at >> 4) : (at >> 7) * 128 + 4 * (at & 31) + ((at >> 5) & 3));
-            const int i = i0 + 4 * l31;
-            if (o < p.out && i < p.blocks * kBlk8) {
-                if constexpr (WN == 4)
-                    *reinterpret_cast<f32x4*>(dst + (int64_t)o * ld + i) = f32x4{acc[m][0][r], acc[m][1][r], acc[m][2][r], acc[m][3][r]};
-                else
+            const int at = 32 * (BM == 64 ? wid >> 1 : wid * WM + m) + (r & 3) + 8 * (r >> 2) + 4 * half;
+            const int o = o0 + W::channel(at), i = i0 + 4 * l31 + (BM == 64 ? 2 * (wid & 1) : 0);
+            if (o >= p.out) continue;
+            if constexpr (WHOLE) {
+                T* const dst = gw + (int64_t)o * p.c + i;
 #pragma unroll
-                    for (int n = 0; n < WN; ++n) dst[(int64_t)o * ld + i + 2 * (wid & 1) + n] = acc[m][n][r];
+                for (int n = 0; n < WN; ++n) {
+                    float one[1] = {alpha * acc[m][n][r]};
+                    if (i + n < p.c) store_vec<DT, 1>(dst + n, one);
+                }
+            } else if (i < ld) {
+                float* const dst = part + ((int64_t)slice * p.out + o) * ld + i;
+                if constexpr (WN == 4) *reinterpret_cast<f32x4*>(dst) = f32x4{acc[m][0][r], acc[m][1][r], acc[m][2][r], acc[m][3][r]};
+                else *reinterpret_cast<f32x2*>(dst) = f32x2{acc[m][0][r], acc[m][1][r]};
             }
         }
     }
-    if (tn == 0 && part_b) {       // the row quads' sums of each channel, added in order
-        __syncthreads();
-        float* const fold = reinterpret_cast<float*>(&As[0][0][0]);          // [kRows / 4][BM]
+    if (tn == 0 && (WHOLE ? gb != nullptr : part_b != nullptr)) {      // the row quads' sums of each channel, added in order
+        constexpr int AG = AR < KR / 4 ? AR : KR / 4;                  // row quads that have one
+        float* const fold = reinterpret_cast<float*>(&cells[0][0]);
+        if (ar < AG)
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            const int e = tid + q * kBlock, oq = e % (BM / 4), rq = e / (BM / 4);
-            if (rq < kRows / 4)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) fold[rq * BM + 4 * oq + j] = sum[q][j];
-        }
+            for (int j = 0; j < 4; ++j) fold[ar * BM + 4 * oq + j] = sum[j];
         __syncthreads();
         for (int o = tid; o < BM; o += kBlock) {
-            float t = fold[o];
-            for (int rq = 1; rq < kRows / 4; ++rq) t += fold[rq * BM + o];
-            if (o0 + o < p.out) part_b[(int64_t)slice * p.out + o0 + o] = t;
+            float t[1] = {fold[o]};
+            for (int rq = 1; rq < AG; ++rq) t[0] += fold[rq * BM + o];
+            if (o0 + o >= p.out) continue;
+            if constexpr (WHOLE) store_vec<DT, 1>(gb + o0 + o, t);
+            else part_b[(int64_t)slice * p.out + o0 + o] = t[0];
         }
     }
 }
 
-// gw[o][i] = alpha * the slices' tiles in order; gb likewise
+// gw[o][i] = alpha * the sum of the slices' tiles; gb likewise.  64 quads of channels a work-group, four threads each: a quarter of
+// the slices in order, the quarters in order behind it.
 template <int DT>
 __global__ __launch_bounds__(kBlock) void linear_wgrad8_reduce_kernel(const float* __restrict__ part, const float* __restrict__ part_b,
                                                                       typename Elem<DT>::T* __restrict__ gw,
                                                                       typename Elem<DT>::T* __restrict__ gb, float alpha, const WgShape p) {
+    __shared__ f32x4 quarter[3][64];
     const int64_t ld = (int64_t)p.blocks * kBlk8, size = (int64_t)p.out * ld;
-    const int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (e < (int64_t)p.out * p.c) {
-        const int64_t o = e / p.c, i = e - o * p.c;
-        float v[1] = {part[o * ld + i]};
-        for (int s = 1; s < p.slices; ++s) v[0] += part[s * size + o * ld + i];
-        v[0] *= alpha;
-        store_vec<DT, 1>(gw + e, v);
+    const int lane = threadIdx.x & 63, part4 = threadIdx.x >> 6;
+    const int64_t e = ((int64_t)blockIdx.x * 64 + lane) * 4;
+    const int per = (p.slices + 3) / 4, first = part4 * per, end = first + per < p.slices ? first + per : p.slices;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (e < size)
+#pragma unroll 8
+        for (int s = first; s < end; ++s) {
+            const f32x4 t = *reinterpret_cast<const f32x4*>(part + s * size + e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += t[j];
+        }
+    if (part4 > 0) quarter[part4 - 1][lane] = v;
+    __syncthreads();
+    if (part4 == 0 && e < size) {
+        const int64_t o = e / ld, i = e - o * ld;
+        float one[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) one[j] = alpha * (((v[j] + quarter[0][lane][j]) + quarter[1][lane][j]) + quarter[2][lane][j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float w[1] = {one[j]};
+            if (i + j < p.c) store_vec<DT, 1>(gw + o * p.c + i + j, w);
+        }
     }
-    if (gb && e < p.out) {
-        float v[1] = {part_b[e]};
-        for (int s = 1; s < p.slices; ++s) v[0] += part_b[(int64_t)s * p.out + e];
-        store_vec<DT, 1>(gb + e, v);
+    const int64_t u = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (gb && u < p.out) {
+        float w[1] = {part_b[u]};
+        for (int s = 1; s < p.slices; ++s) w[0] += part_b[(int64_t)s * p.out + u];
+        store_vec<DT, 1>(gb + u, w);
     }
 }
 
@@ -273,23 +461,48 @@ __global__ __launch_bounds__(kBlock) void fill_zero_kernel(typename Elem<DT>::T*
     if (gb && e < out) gb[e] = 0;
 }
 
-int wg_tile(int64_t out) { return out <= 64 ? 64 : out <= 128 ? 128 : 256; }
+int wg_rows(int32_t dtype) { return dtype == SAE_F32 ? 32 : 64; }      // WgTile::KR
 
-WgShape wg_plan(int64_t rows, int64_t out, int64_t c) {
+struct WgPlan {
+    int bm;
     WgShape p;
-    p.rows = rows;
-    p.out = (int)out;
-    p.c = (int)c;
-    p.blocks = (int)ceil_div64(c, kBlk8);
-    p.tiles_m = (int)ceil_div64(out, wg_tile(out));
-    p.tiles_n = (int)ceil_div64(c, kBN);
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, steps = ceil_div64(rows, kRows);
-    int64_t s = ceil_div64(512, tiles);                  // two work-groups per CU
-    if (s > steps) s = steps;
-    if (s < 1) s = 1;
-    p.slice_rows = ceil_div64(steps, s) * kRows;
-    p.slices = (int)ceil_div64(rows, p.slice_rows);
-    return p;
+};
+
+// The tallest tile that still gives every CU a work-group of at least two steps a wave group, 64 if none does; slices so that the
+// work-groups fill the 256 CUs in as few rounds as the work allows.
+WgPlan wg_plan(int64_t rows, int64_t out, int64_t c, int32_t dtype) {
+    const int kr = wg_rows(dtype);
+    const int64_t steps = ceil_div64(rows, kr), pairs = ceil_div64(steps, 4), tiles_n = ceil_div64(c, kBN);
+    int bm = 64;
+    for (int t : {256, 128})
+        if (out > t / 2 && ceil_div64(out, t) * tiles_n * pairs >= 256) { bm = t; break; }
+    if (const int forced = tuning_knob("SAE_WG_TILE", 0)) bm = forced;      // (tests: every height at small sizes)
+    WgPlan w;
+    w.bm = bm;
+    w.p.rows = rows;
+    w.p.out = (int)out;
+    w.p.c = (int)c;
+    w.p.blocks = (int)ceil_div64(c, kBlk8);
+    w.p.tiles_m = (int)ceil_div64(out, bm);
+    w.p.tiles_n = (int)tiles_n;
+    const int64_t tiles = ceil_div64(out, bm) * tiles_n;
+    int64_t best = 1;
+    if (tiles < 256) {
+        best = 256 / tiles;
+        if (best > 8) best = best / 8 * 8;
+    }
+    if (best > pairs) best = pairs;
+    // a slice's rows lie behind one descriptor with 32-bit offsets
+    const int64_t widest = ceil_div64(c, kBlk8) * kBlk8 > 4 * out ? ceil_div64(c, kBlk8) * kBlk8 : 4 * out;
+    const int64_t least = ceil_div64(rows, ((int64_t)1 << 30) / widest / kr * kr);
+    if (best < least) best = least;
+    w.p.slice_rows = ceil_div64(steps, best) * kr;
+    w.p.slices = (int)ceil_div64(rows, w.p.slice_rows);
+    return w;
+}
+
+int64_t wg_workspace(const WgPlan& w) {
+    return w.p.slices == 1 ? 0 : (int64_t)w.p.slices * w.p.out * ((int64_t)w.p.blocks * kBlk8 + 1);
 }
 
 bool wg_shape_ok(int64_t rows, int64_t out, int64_t c) {
@@ -297,13 +510,17 @@ bool wg_shape_ok(int64_t rows, int64_t out, int64_t c) {
            rows <= ((int64_t)1 << 40) / (out + c);
 }
 
-template <int DT, int BM>
-void wg_launch(const void* gy, const int8_t* codes, const uint8_t* scales, float* part, float* part_b, const WgShape& p, bool vec,
-               hipStream_t s) {
+template <int DT, int BM, bool VEC>
+void wg_launch(const void* gy, const int8_t* codes, const uint8_t* scales, float* part, float* part_b, void* gw, void* gb, float alpha,
+               const WgShape& p, hipStream_t s) {
     using T = typename Elem<DT>::T;
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n * p.slices)), block(kBlock);
-    if (vec) hipLaunchKernelGGL((linear_wgrad8_kernel<DT, BM, true>), grid, block, 0, s, (const T*)gy, codes, scales, part, part_b, p);
-    else hipLaunchKernelGGL((linear_wgrad8_kernel<DT, BM, false>), grid, block, 0, s, (const T*)gy, codes, scales, part, part_b, p);
+    if (p.slices == 1)
+        hipLaunchKernelGGL((linear_wgrad8_kernel<DT, BM, VEC, true>), grid, block, 0, s, (const T*)gy, codes, scales, part, part_b,
+                           (T*)gw, (T*)gb, alpha, p);
+    else
+        hipLaunchKernelGGL((linear_wgrad8_kernel<DT, BM, VEC, false>), grid, block, 0, s, (const T*)gy, codes, scales, part, part_b,
+                           (T*)gw, (T*)gb, alpha, p);
 }
 
 template <int DT>
@@ -315,16 +532,20 @@ int wg_run(const void* gy, const int8_t* codes, const uint8_t* scales, void* gw,
                            out * c, out);
         return check_launch("sae_linear_wgrad8");
     }
-    const WgShape p = wg_plan(rows, out, c);
+    const WgPlan w = wg_plan(rows, out, c, DT);
+    const WgShape& p = w.p;
     const bool vec = out % 4 == 0 && reinterpret_cast<uintptr_t>(gy) % (4 * sizeof(T)) == 0;
     float* part_b = gb ? ws + (int64_t)p.slices * out * p.blocks * kBlk8 : nullptr;
-    switch (wg_tile(out)) {
-        case 64: wg_launch<DT, 64>(gy, codes, scales, ws, part_b, p, vec, s); break;
-        case 128: wg_launch<DT, 128>(gy, codes, scales, ws, part_b, p, vec, s); break;
-        default: wg_launch<DT, 256>(gy, codes, scales, ws, part_b, p, vec, s); break;
-    }
-    hipLaunchKernelGGL((linear_wgrad8_reduce_kernel<DT>), dim3((unsigned)ceil_div64(out * c, kBlock)), dim3(kBlock), 0, s,
-                       (const float*)ws, (const float*)part_b, (T*)gw, (T*)gb, alpha, p);
+#define SAE_WG(BM)                                                                                                              \
+    if (vec) wg_launch<DT, BM, true>(gy, codes, scales, ws, part_b, gw, gb, alpha, p, s);                                       \
+    else wg_launch<DT, BM, false>(gy, codes, scales, ws, part_b, gw, gb, alpha, p, s)
+    if (w.bm == 64) { SAE_WG(64); }
+    else if (w.bm == 128) { SAE_WG(128); }
+    else { SAE_WG(256); }
+#undef SAE_WG
+    if (p.slices > 1)
+        hipLaunchKernelGGL((linear_wgrad8_reduce_kernel<DT>), dim3((unsigned)ceil_div64(out * p.blocks * kBlk8, 256)),
+                           dim3(kBlock), 0, s, (const float*)ws, (const float*)part_b, (T*)gw, (T*)gb, alpha, p);
     return check_launch("sae_linear_wgrad8");
 }
 
@@ -333,10 +554,9 @@ int wg_run(const void* gy, const int8_t* codes, const uint8_t* scales, void* gw,
 
 using namespace sae;
 
-extern "C" int64_t sae_linear_wgrad8_workspace(int64_t rows, int64_t out, int64_t c) {
-    if (!wg_shape_ok(rows, out, c) || rows == 0) return 0;
-    const WgShape p = wg_plan(rows, out, c);
-    return (int64_t)p.slices * out * ((int64_t)p.blocks * kBlk8 + 1);
+extern "C" int64_t sae_linear_wgrad8_workspace(int64_t rows, int64_t out, int64_t c, int32_t dtype) {
+    if (!wg_shape_ok(rows, out, c) || !elem_known(dtype) || rows == 0) return 0;
+    return wg_workspace(wg_plan(rows, out, c, dtype));
 }
 
 extern "C" int sae_linear_wgrad8(const void* gy, const int8_t* codes, const uint8_t* scales, void* gw, void* gb, int64_t rows,
@@ -348,9 +568,10 @@ extern "C" int sae_linear_wgrad8(const void* gy, const int8_t* codes, const uint
     if (!gw || (rows > 0 && (!gy || !codes || !scales))) return fail(SAE_EINVAL, "sae_linear_wgrad8: null tensor");
     if (rows > 0 && (!aligned16(codes) || !aligned16(workspace) || reinterpret_cast<uintptr_t>(gy) % (uintptr_t)elem_bytes(dtype)))
         return fail(SAE_EINVAL, "sae_linear_wgrad8: misaligned tensor");
-    if (rows > 0 && (!workspace || workspace_floats < sae_linear_wgrad8_workspace(rows, out, c)))
+    const int64_t need = sae_linear_wgrad8_workspace(rows, out, c, dtype);
+    if (need > 0 && (!workspace || workspace_floats < need))
         return fail(SAE_EWORKSPACE, "sae_linear_wgrad8: workspace %lld < %lld floats (sae_linear_wgrad8_workspace)",
-                    (long long)workspace_floats, (long long)sae_linear_wgrad8_workspace(rows, out, c));
+                    (long long)workspace_floats, (long long)need);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == SAE_F32) return wg_run<SAE_F32>(gy, codes, scales, gw, gb, rows, out, c, alpha, workspace, s);
     if (dtype == SAE_BF16) return wg_run<SAE_BF16>(gy, codes, scales, gw, gb, rows, out, c, alpha, workspace, s);

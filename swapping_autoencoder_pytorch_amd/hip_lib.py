@@ -132,7 +132,7 @@ _SIGNATURES = {
                                  _f32, _i32, _f32, _f32, _i32, C.c_void_p, _i64, _stream]),
     "group_norm_act_bwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, _f32p, _f32p, _f32p, _f32p, C.c_void_p, _f32p,
                                      _f32p, _i64, _i64, _i64, _i64, _i32, _f32, _f32, _i32, C.c_void_p, _i64, _stream]),
-    "linear_wgrad8_workspace": (_i64, [_i64, _i64, _i64]),
+    "linear_wgrad8_workspace": (_i64, [_i64, _i64, _i64, _i32]),
     "linear_wgrad8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, _i64, _i64, _i64, _f32, _i32, _f32p,
                                 _i64, _stream]),
 }

@@ -104,7 +104,7 @@ def linear_weight_grad8(gy, kept, bias=True, alpha=1.0):
     out, c = gy.shape[-1], kept.channels
     gw = torch.empty(out, c, dtype=gy.dtype, device=gy.device)
     gb = torch.empty(out, dtype=gy.dtype, device=gy.device) if bias else None
-    n_ws = lib.query("linear_wgrad8_workspace", kept.rows, out, c)
+    n_ws = lib.query("linear_wgrad8_workspace", kept.rows, out, c, hip_lib.element_types()[gy.dtype])
     ws = torch.empty(max(n_ws, 1), dtype=torch.float32, device=gy.device)
     with lib.device_of(gy):
         lib.call("linear_wgrad8", gy.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), gw.data_ptr(), hip_lib.ptr(gb),

@@ -231,3 +231,17 @@ def check_wgrad(device, dtype, shape, alpha=1.0, bias=True):
         return
     assert gb.dtype == dtype and tuple(gb.shape) == (out,)
     assert ((gb.cpu().double() - g.sum(0)).abs() <= 2 * E32 * (rows + 32) * g.abs().sum(0) * (1 + u) + u * g.sum(0).abs() + 1e-30).all()
+
+
+def check_wgrad_on_device(device, dtype, shape):
+    """check_wgrad at sizes where the reference is computed on the device as well (its own float64 products)"""
+    from swapping_autoencoder_pytorch_amd.stylegan2_op import checkpoint8, linear_weight_grad8
+    rows, c, out = shape
+    x, gy = seeded((rows, c), 20, dtype, 0.2).to(device), seeded((rows, out), 21, dtype, 0.0, 0.3).to(device)
+    kept = checkpoint8(x)
+    gw, gb = linear_weight_grad8(gy, kept)
+    v, g, u = kept.dequantize().double(), gy.double().t().contiguous(), half_step(dtype)
+    want, size = g @ v, g.abs() @ v.abs()
+    assert ((gw.double() - want).abs() <= 2 * E32 * (rows + 32) * size * (1 + u) + u * want.abs()).all()
+    want, size = g.sum(1), g.abs().sum(1)
+    assert ((gb.double() - want).abs() <= 2 * E32 * (rows + 32) * size * (1 + u) + u * want.abs()).all()

@@ -80,11 +80,15 @@ def test_entry_points_refuse(emu_lib):
             args = bad if name.endswith("_pack") and not name.endswith("unpack") else [bad[1], bad[2], bad[0]] + bad[3:]
             with pytest.raises(hip_lib.SaeError):
                 emu_lib.call(name, *args)
-    n = emu_lib.query("linear_wgrad8_workspace", 4, 16, 16)
+    rows = 600                                       # several slices: with a workspace
+    n = emu_lib.query("linear_wgrad8_workspace", rows, 16, 16, 0)
+    assert n > 0 and emu_lib.query("linear_wgrad8_workspace", 4, 16, 16, 0) == 0
+    gy, codes, scales = torch.zeros(rows, 16), torch.zeros(rows, 32, dtype=torch.int8), torch.full((1, rows), 127, dtype=torch.uint8)
     wsf, gw = torch.empty(n), torch.empty(16, 16)
-    good = [p(x), p(codes), p(scales), p(gw), None, 4, 16, 16, 1.0, 0, p(wsf), n, None]
+    good = [p(gy), p(codes), p(scales), p(gw), None, rows, 16, 16, 1.0, 0, p(wsf), n, None]
+    emu_lib.call("linear_wgrad8", *good)
     for at, value in ((0, None), (1, None), (2, None), (3, None), (5, -1), (6, 0), (7, 0), (9, 3), (10, None), (11, n - 1), (1, p(codes) + 4),
-                      (0, p(x) + 2)):
+                      (0, p(gy) + 2)):
         bad = list(good)
         bad[at] = value
         with pytest.raises(hip_lib.SaeError):
@@ -307,6 +311,16 @@ def check_context(device):
         assert ga.shape == t.shape and ((ga - 2 * t).abs() <= t.abs().max() * 2.0 ** -5).all()
 
 
+@pytest.mark.parametrize("tile", [64, 128, 256])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_wgrad_every_tile_emulated(emu_lib, dtype, tile, monkeypatch):
+    """the tile heights that small sizes do not reach by themselves (the knob exists in tuning builds only)"""
+    monkeypatch.setenv("SAE_WG_TILE", str(tile))
+    with backend(emu_lib):
+        for shape in ((70, 130, 300), (33, 40, 7), (300, 64, 129)):
+            K.check_wgrad("cpu", K.TYPES[dtype], shape)
+
+
 CHECKS = [check_memory_orders, check_empty, check_not_finite, check_linear8, check_run_together, check_context]
 
 
@@ -339,6 +353,14 @@ def test_gpu_norm(dtype, shape):
 def test_gpu_wgrad(dtype, shape):
     K.check_wgrad("cuda:0", K.TYPES[dtype], shape)
     K.check_wgrad("cuda:0", K.TYPES[dtype], shape, alpha=-0.37, bias=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2000, 640, 1100), (4100, 1030, 2048), (1025, 2048, 513), (20000, 256, 250)], ids=lambda s: "r%d_c%d_o%d" % s)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_wgrad_large(dtype, shape):
+    """sizes that fill the chip: the tall tiles, slices for every XCD"""
+    K.check_wgrad_on_device("cuda:0", K.TYPES[dtype], shape)
 
 
 @pytest.mark.gpu
