@@ -23,12 +23,13 @@ __global__ __launch_bounds__(kBlock) void checkpoint8_pack_kernel(const typename
         const bool live = block < rows * blocks;      // (whole groups of LB lanes are live or not)
         const int64_t row = live ? block / blocks : 0, cb = live ? block - row * blocks : 0;
         const int64_t col = cb * kBlk8 + (int64_t)(threadIdx.x % LB) * V;
-        float v[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = 0.0f;
-        if (live && col < c) load_vec<DT, V>(x + row * c + col, v);
-        const unsigned e = block8_exponent<DT>(block8_amax<LB>(vec_amax<V>(v)));
+        Raw<DT, V> raw;
+        raw.zero();
+        if (live && col < c) raw.load(x + row * c + col);
+        const unsigned e = block8_exponent<DT>(block8_amax<LB>(raw.amax()));
         if (!live) continue;
+        float v[V];
+        raw.get(v);
         store_codes<V>(codes + row * blocks * kBlk8 + col, v, block8_inverse(e));
         if (threadIdx.x % LB == 0) scales[cb * rows + row] = (uint8_t)e;
     }
@@ -45,8 +46,10 @@ __global__ __launch_bounds__(kBlock) void checkpoint8_unpack_kernel(const int8_t
         const int64_t row = block / blocks, cb = block - row * blocks;
         const int64_t col = cb * kBlk8 + (int64_t)(threadIdx.x % LB) * V;
         if (col >= c) continue;
+        RawCodes<V> raw;
+        raw.load(codes + row * blocks * kBlk8 + col);
         float v[V];
-        load_codes<V>(codes + row * blocks * kBlk8 + col, block8_step(scales[cb * rows + row]), v);
+        raw.get(block8_step(scales[cb * rows + row]), v);
         store_vec<DT, V>(x + row * c + col, v);
     }
 }

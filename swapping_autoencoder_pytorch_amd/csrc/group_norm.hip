@@ -10,8 +10,11 @@
 // Every statistic needs the whole group before the first result can be written, so each direction walks its tensors twice:
 //     sums      per (sample, chunk of rows, channel), in registers, one record per chunk
 //     totals    the chunks' records added in order: mean / rstd, or m1 / m2 and the channel sums
-//     apply     the elementwise pass
-// All of them are HBM-bound: forward 2 reads + 1 write (the floor is 1 + 1), backward 4 + 1 (2 + 1).
+//     apply     the elementwise pass, last chunk first: what the sums read last is what the caches still hold
+// or, where a sample's groups are small, all of it in one work-group per (sample, slab of whole groups): one launch.
+//
+// Layout of a walk: a lane owns V neighbouring channels (16 bytes) and takes four rows at a time, so that four loads are under way
+// and the exponents of four rows are one word.
 //
 // Numerics: a thread adds x - x0 and (x - x0)^2 over its rows, x0 the first value it meets in the channel: at most the number of
 // its rows times the rounding of a plain sum, whatever the channel's mean.  The records are moments about zero in 64 bits, which
@@ -21,17 +24,21 @@
 namespace sae {
 namespace {
 
+constexpr int kQ = 4;              // rows a thread takes at a time
+constexpr int kFused = 512;        // most threads of a one-launch work-group
+
 struct GnShape {
     int64_t l;                 // positions of a sample
     int64_t rows;              // n * l: rows of codes, stride of a block's exponents
     int c, groups, cg;
-    int lanes;                 // channel vectors of a row, padded to whole 8-bit blocks
-    int tile;                  // lanes a work-group covers at a time: min(lanes, kBlock)
-    int rp;                    // rows it covers at a time: kBlock / tile
+    int lanes;                 // channel vectors of a row (of a slab), padded to whole 8-bit blocks
+    int tile;                  // lanes a work-group covers at a time
+    int rp;                    // rows it covers at a time: threads / tile, kQ of each
     int chunk_rows;            // rows of a work-group
     int chunks;                // chunks of a sample
     int units;                 // records of a chunk: channel vectors if a vector lies in one group, channels if not
     int blocks;                // 8-bit blocks of a row
+    int slab, slabs;           // groups of a one-launch work-group (0: not that form), slabs of a sample
 };
 
 #ifdef HIPEMU
@@ -42,96 +49,205 @@ __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float rcp_fast(float v) { return __builtin_amdgcn_rcpf(v); }      // 1 ulp
 #endif
 
-// 1 / (1 + exp(-z)); z -> -infinity: exp2 gives infinity and the quotient 0
-__device__ __forceinline__ float sigmoid_f(float z) { return rcp_fast(1.0f + exp2_fast(z * -1.44269504088896341f)); }
+// Activations of t = kArg * z (SiLU's exponent has base 2, so its factor goes into the affine map in front):
+//   value   act(z) * scale;      slope   act'(z)
+template <int ACT>
+struct Act {
+    static constexpr float kArg = ACT == SAE_ACT_SILU ? 1.44269504088896341f : 1.0f;
+    static constexpr float kLn2 = 0.693147180559945309f;
+    // z -> -infinity: exp2 gives infinity and the quotient 0
+    static __device__ __forceinline__ float sigmoid(float t) { return rcp_fast(1.0f + exp2_fast(-t)); }
+    static __device__ __forceinline__ float value(float t, float slope, float scale) {
+        if constexpr (ACT == SAE_ACT_LRELU) return t * (t > 0.0f ? scale : scale * slope);
+        else if constexpr (ACT == SAE_ACT_SILU) return t * (kLn2 * scale) * sigmoid(t);
+        else return t * scale;
+    }
+    static __device__ __forceinline__ float derivative(float t, float slope) {
+        if constexpr (ACT == SAE_ACT_LRELU) return t > 0.0f ? 1.0f : slope;
+        else if constexpr (ACT == SAE_ACT_SILU) {
+            const float s = sigmoid(t);
+            return s * fmaf(t, fmaf(-kLn2, s, kLn2), 1.0f);
+        } else return 1.0f;
+    }
+};
 
-template <int ACT>
-__device__ __forceinline__ float act_f(float z, float slope) {
-    if constexpr (ACT == SAE_ACT_LRELU) return z > 0.0f ? z : z * slope;
-    else if constexpr (ACT == SAE_ACT_SILU) return z * sigmoid_f(z);
-    else return z;
+// The groups of a lane's V channels, one division for all of them
+template <int V>
+__device__ __forceinline__ void groups_of(int c0, int cg, int (&g)[V]) {
+    int at = c0 / cg, left = cg - (c0 - at * cg);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        g[j] = at;
+        if (--left == 0) { ++at; left = cg; }
+    }
 }
-template <int ACT>
-__device__ __forceinline__ float act_slope_f(float z, float slope) {
-    if constexpr (ACT == SAE_ACT_LRELU) return z > 0.0f ? 1.0f : slope;
-    else if constexpr (ACT == SAE_ACT_SILU) {
-        const float s = sigmoid_f(z);
-        return s * fmaf(z, 1.0f - s, 1.0f);
-    } else return 1.0f;
+
+// V neighbours of a parameter (absent: all `none`)
+template <int V>
+__device__ __forceinline__ void load_param(const float* __restrict__ w, int c0, float none, float (&v)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = none;
+    if (!w) return;
+    if constexpr (V >= 4) __builtin_memcpy(v, w + c0, sizeof(v));
+    else v[0] = w[c0];
+}
+
+// Where a thread stands in a walk over rows [r_begin, r_end) of sample n
+struct Walk {
+    int tx, ty, c0, rp;
+    int64_t first, r_end, row0;        // row0: the sample's first row
+    bool mine;                         // the lane has channels
+};
+
+// sum over ty of the threads' values (red[ty * width + tx], every thread's written): at red[tx] behind it, in a fixed order
+template <typename P>
+__device__ __forceinline__ void fold_rows(P* red, int tx, int ty, int width, int rp, bool on) {
+    int half = 1;
+    while (half < rp) half <<= 1;
+    for (half >>= 1; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (on && ty < half && ty + half < rp) {
+            P& a = red[ty * width + tx];
+            const P b = red[(ty + half) * width + tx];
+            a.x += b.x;
+            a.y += b.y;
+        }
+    }
+    __syncthreads();
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 
-// record [n][chunk][unit]: sum x and sum x^2 of the unit over the chunk's rows
+// a thread's moments over its rows, and (KEEP) the checkpoint of them; every thread of the work-group makes the same trips
 template <int DT, int V, bool KEEP>
-__global__ __launch_bounds__(kBlock) void gn_sums_kernel(const typename Elem<DT>::T* __restrict__ x, double2* __restrict__ rec,
-                                                         int8_t* __restrict__ codes, uint8_t* __restrict__ scales, const GnShape p) {
+__device__ __forceinline__ void walk_sums(const typename Elem<DT>::T* __restrict__ x, int8_t* __restrict__ codes,
+                                          uint8_t* __restrict__ scales, const Walk& w, const GnShape& p, double (&sx)[V], double (&sxx)[V]) {
     constexpr int LB = kBlk8 / V;
-    __shared__ double2 red[kBlock * V];
-    const int n = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
-    const int tx = tid % p.tile, ty = tid / p.tile;
-    const int64_t r_begin = (int64_t)chunk * p.chunk_rows;
-    const int64_t r_end = r_begin + p.chunk_rows < p.l ? r_begin + p.chunk_rows : p.l;
-    const bool whole = p.cg % V == 0;
-    for (int lane0 = 0; lane0 < p.lanes; lane0 += p.tile) {
-        const int c0 = (lane0 + tx) * V;
-        const bool live = ty < p.rp && c0 < p.c;
-        float k[V], s1[V], s2[V];
+    float k[V], s1[V], s2[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) k[j] = s1[j] = s2[j] = 0.0f;
-        int64_t count = 0;
-        if (live && r_begin + ty < r_end) load_vec<DT, V>(x + ((int64_t)n * p.l + r_begin + ty) * p.c + c0, k);
-        // (every lane of a work-group makes the same trips: the blocks' lanes meet in shuffles)
-        for (int64_t r0 = r_begin; r0 < r_end; r0 += p.rp) {
-            const int64_t r = r0 + ty;
-            const bool on = live && r < r_end;
+    for (int j = 0; j < V; ++j) k[j] = s1[j] = s2[j] = 0.0f;
+    const int64_t begin = w.first + kQ * w.ty;
+    if (w.mine && begin < w.r_end) {
+        Raw<DT, V> raw;
+        raw.load(x + (w.row0 + begin) * p.c + w.c0);
+        raw.get(k);
+    }
+    int64_t count = 0;
+    const int cb = w.c0 / kBlk8;
+    const bool kept = KEEP && w.ty < w.rp && cb < p.blocks;
+    for (int64_t r0 = w.first; r0 < w.r_end; r0 += kQ * w.rp) {
+        const int64_t r = r0 + kQ * w.ty;
+        Raw<DT, V> raw[kQ];
+        const int have = !w.mine || r >= w.r_end ? 0 : w.r_end - r < kQ ? (int)(w.r_end - r) : kQ;
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {
+            raw[i].zero();
+            if (i < have) raw[i].load(x + (w.row0 + r + i) * p.c + w.c0);
+        }
+        unsigned e[kQ];
+        if constexpr (KEEP)
+#pragma unroll
+            for (int i = 0; i < kQ; ++i) e[i] = block8_exponent<DT>(block8_amax<LB>(raw[i].amax()));
+        count += have;
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {
             float v[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = 0.0f;
-            if (on) {
-                load_vec<DT, V>(x + ((int64_t)n * p.l + r) * p.c + c0, v);
-                ++count;
+            raw[i].get(v);
+            if (i < have)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float d = v[j] - k[j];
                     s1[j] += d;
                     s2[j] = fmaf(d, d, s2[j]);
                 }
-            }
-            if constexpr (KEEP) {
-                const unsigned e = block8_exponent<DT>(block8_amax<LB>(vec_amax<V>(v)));
-                const int cb = (lane0 + tx) / LB;
-                const int64_t row = (int64_t)n * p.l + r;
-                if (ty < p.rp && cb < p.blocks && r < r_end) {
-                    store_codes<V>(codes + row * p.blocks * kBlk8 + c0, v, block8_inverse(e));
-                    if ((lane0 + tx) % LB == 0) scales[(int64_t)cb * p.rows + row] = (uint8_t)e;
+            if constexpr (KEEP)
+                if (kept && r + i < w.r_end) store_codes<V>(codes + (w.row0 + r + i) * p.blocks * kBlk8 + w.c0, v, block8_inverse(e[i]));
+        }
+        if constexpr (KEEP)
+            if (kept && w.c0 % kBlk8 == 0) {
+                uint8_t* to = scales + (int64_t)cb * p.rows + w.row0 + r;
+                if (r + kQ <= w.r_end) {
+                    const unsigned word = e[0] | (e[1] << 8) | (e[2] << 16) | (e[3] << 24);
+                    __builtin_memcpy(to, &word, 4);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kQ; ++i)
+                        if (r + i < w.r_end) to[i] = (uint8_t)e[i];
                 }
             }
-        }
-        // moments about zero, then the sum over the rows' threads
-        __syncthreads();
-        const double m = (double)count;
-        double a = 0.0, b = 0.0;
+    }
+    const double m = (double)count;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {                                  // about zero
+        const double kd = k[j], d1 = s1[j];
+        sx[j] = m * kd + d1;
+        sxx[j] = (double)s2[j] + 2.0 * kd * d1 + m * kd * kd;
+    }
+}
+
+// mean and rstd of m values from their moments about zero
+__device__ __forceinline__ float2 moments(double a, double b, double m, float eps) {
+    const double mu = a / m;
+    double var = b / m - mu * mu;
+    if (var < 0.0) var = 0.0;                                      // (a NaN stays one)
+    return float2{(float)mu, (float)(1.0 / sqrt(var + (double)eps))};
+}
+
+template <int DT, int V, int ACT, bool STREAM>
+__device__ __forceinline__ void walk_apply(const typename Elem<DT>::T* __restrict__ x, typename Elem<DT>::T* __restrict__ y, const Walk& w,
+                                           const GnShape& p, const float (&mu)[V], const float (&a)[V], const float (&b)[V], float slope,
+                                           float scale) {
+    for (int64_t r = w.first + kQ * w.ty; r < w.r_end; r += kQ * w.rp) {
+        const int64_t at = (w.row0 + r) * p.c + w.c0;
+        const int have = w.r_end - r < kQ ? (int)(w.r_end - r) : kQ;
+        Raw<DT, V> raw[kQ];
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            if (i < have) raw[i].load(x + at + (int64_t)i * p.c);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            if (i < have) {
+                float v[V];
+                raw[i].get(v);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = Act<ACT>::value(fmaf(v[j] - mu[j], a[j], b[j]), slope, scale);
+                store_vec<DT, V, STREAM>(y + at + (int64_t)i * p.c, v);
+            }
+    }
+}
+
+// record [n][chunk][unit]: sum x and sum x^2 of the unit over the chunk's rows
+template <int DT, int V, bool KEEP>
+__global__ __launch_bounds__(kBlock) void gn_sums_kernel(const typename Elem<DT>::T* __restrict__ x, double2* __restrict__ rec,
+                                                         int8_t* __restrict__ codes, uint8_t* __restrict__ scales, const GnShape p) {
+    __shared__ double2 red[kBlock];
+    const int n = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
+    Walk w;
+    w.tx = tid % p.tile;
+    w.ty = tid / p.tile;
+    w.rp = p.rp;
+    w.row0 = (int64_t)n * p.l;
+    w.first = (int64_t)chunk * p.chunk_rows;
+    w.r_end = w.first + p.chunk_rows < p.l ? w.first + p.chunk_rows : p.l;
+    const bool whole = p.cg % V == 0;
+    for (int lane0 = 0; lane0 < p.lanes; lane0 += p.tile) {
+        w.c0 = (lane0 + w.tx) * V;
+        w.mine = w.ty < w.rp && w.c0 < p.c;
+        double sx[V], sxx[V];
+        walk_sums<DT, V, KEEP>(x, codes, scales, w, p, sx, sxx);
+        const int rounds = whole ? 1 : V;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const double kd = k[j], d1 = s1[j];
-            const double sx = m * kd + d1, sxx = (double)s2[j] + 2.0 * kd * d1 + m * kd * kd;
-            if (whole) { a += sx; b += sxx; }
-            else red[tid * V + j] = double2{sx, sxx};
-        }
-        if (whole) red[tid] = double2{a, b};
-        __syncthreads();
-        const int per = whole ? 1 : V;
-        for (int u = tid; u < p.tile * per; u += kBlock) {
-            const int unit = lane0 * per + u;
-            if (unit >= p.units) continue;
-            double2 t = red[u];
-            for (int y = 1; y < p.rp; ++y) {
-                const double2 o = red[y * p.tile * per + u];
-                t.x += o.x;
-                t.y += o.y;
-            }
-            rec[((int64_t)n * p.chunks + chunk) * p.units + unit] = t;
+            if (j >= rounds) break;
+            double2 t{sx[j], sxx[j]};
+            if (whole)
+#pragma unroll
+                for (int i = 1; i < V; ++i) { t.x += sx[i]; t.y += sxx[i]; }
+            __syncthreads();
+            red[tid] = t;
+            fold_rows(red, w.tx, w.ty, p.tile, p.rp, w.ty < p.rp);
+            const int unit = whole ? lane0 + w.tx : w.c0 + j;
+            if (w.ty == 0 && w.c0 < p.c) rec[((int64_t)n * p.chunks + chunk) * p.units + unit] = red[w.tx];
         }
     }
 }
@@ -157,159 +273,366 @@ __global__ __launch_bounds__(kWave) void gn_totals_kernel(const double2* __restr
     a = wave_sum_d(a);
     b = wave_sum_d(b);
     if (threadIdx.x == 0) {
-        const double m = (double)p.l * p.cg, mu = a / m;
-        double var = b / m - mu * mu;
-        if (var < 0.0) var = 0.0;            // (a NaN stays one)
-        mean[(int64_t)n * p.groups + g] = (float)mu;
-        rstd[(int64_t)n * p.groups + g] = (float)(1.0 / sqrt(var + (double)eps));
+        const float2 s = moments(a, b, (double)p.l * p.cg, eps);
+        mean[(int64_t)n * p.groups + g] = s.x;
+        rstd[(int64_t)n * p.groups + g] = s.y;
     }
 }
 
-template <int DT, int V, int ACT>
-__global__ __launch_bounds__(kBlock) void gn_apply_kernel(const typename Elem<DT>::T* __restrict__ x, const float* __restrict__ mean,
-                                                          const float* __restrict__ rstd, const float* __restrict__ weight,
-                                                          const float* __restrict__ bias, typename Elem<DT>::T* __restrict__ y,
-                                                          float slope, float scale, const GnShape p) {
-    const int n = blockIdx.y, tid = threadIdx.x;
-    const int tx = tid % p.tile, ty = tid / p.tile;
-    const int64_t r_begin = (int64_t)blockIdx.x * p.chunk_rows;
-    const int64_t r_end = r_begin + p.chunk_rows < p.l ? r_begin + p.chunk_rows : p.l;
-    if (ty >= p.rp) return;
+// TOTALS: the statistics too, from the sample's records -- each work-group for itself, where they are few
+constexpr int kFoldGroups = 256, kFoldRecords = 1024;
+template <int DT, int V, int ACT, bool TOTALS>
+__global__ __launch_bounds__(kBlock) void gn_apply_kernel(const typename Elem<DT>::T* __restrict__ x, const double2* __restrict__ rec,
+                                                          float* __restrict__ mean, float* __restrict__ rstd,
+                                                          const float* __restrict__ weight, const float* __restrict__ bias,
+                                                          typename Elem<DT>::T* __restrict__ y, float eps, float slope, float scale,
+                                                          const GnShape p) {
+    const int n = (int)gridDim.y - 1 - (int)blockIdx.y, chunk = (int)gridDim.x - 1 - (int)blockIdx.x, tid = threadIdx.x;
+    Walk w;
+    w.tx = tid % p.tile;
+    w.ty = tid / p.tile;
+    w.rp = p.rp;
+    w.row0 = (int64_t)n * p.l;
+    w.first = (int64_t)chunk * p.chunk_rows;
+    w.r_end = w.first + p.chunk_rows < p.l ? w.first + p.chunk_rows : p.l;
+    __shared__ float2 stat[TOTALS ? kFoldGroups : 1];
+    __shared__ double2 share[TOTALS ? kBlock : 1];
+    if constexpr (TOTALS) {
+        // `per` threads a group (a power of two) take its records in turn, then one adds their shares: the same order in every group
+        const int units = p.units / p.groups, items = p.chunks * units;
+        int per = kBlock;
+        while (per * p.groups > kBlock) per >>= 1;
+        const int g = tid / per, k = tid - g * per;
+        double2 t{0.0, 0.0};
+        if (g < p.groups)
+            for (int i = k; i < items; i += per) {
+                const int at = i / units, u = i - at * units;
+                const double2 o = rec[((int64_t)n * p.chunks + at) * p.units + g * units + u];
+                t.x += o.x;
+                t.y += o.y;
+            }
+        share[tid] = t;
+        __syncthreads();
+        if (g < p.groups && k == 0) {
+            for (int i = 1; i < per; ++i) {
+                t.x += share[tid + i].x;
+                t.y += share[tid + i].y;
+            }
+            const float2 s = moments(t.x, t.y, (double)p.l * p.cg, eps);
+            stat[g] = s;
+            if (chunk == 0) {
+                mean[(int64_t)n * p.groups + g] = s.x;
+                rstd[(int64_t)n * p.groups + g] = s.y;
+            }
+        }
+        __syncthreads();
+    }
+    if (w.ty >= w.rp) return;
     for (int lane0 = 0; lane0 < p.lanes; lane0 += p.tile) {
-        const int c0 = (lane0 + tx) * V;
-        if (c0 >= p.c) return;
+        w.c0 = (lane0 + w.tx) * V;
+        if (w.c0 >= p.c) return;
         float mu[V], a[V], b[V];
+        int g[V];
+        groups_of<V>(w.c0, p.cg, g);
+        load_param<V>(weight, w.c0, 1.0f, a);
+        load_param<V>(bias, w.c0, 0.0f, b);
+        float2 s;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int64_t g = (int64_t)n * p.groups + (c0 + j) / p.cg;
-            mu[j] = mean[g];
-            a[j] = rstd[g] * (weight ? weight[c0 + j] : 1.0f);
-            b[j] = bias ? bias[c0 + j] : 0.0f;
+            if (j == 0 || g[j] != g[j - 1]) {
+                if constexpr (TOTALS) s = stat[g[j]];
+                else s = float2{mean[(int64_t)n * p.groups + g[j]], rstd[(int64_t)n * p.groups + g[j]]};
+            }
+            mu[j] = s.x;
+            a[j] *= s.y * Act<ACT>::kArg;
+            b[j] *= Act<ACT>::kArg;
         }
-        for (int64_t r = r_begin + ty; r < r_end; r += p.rp) {
-            const int64_t at = ((int64_t)n * p.l + r) * p.c + c0;
-            float v[V];
-            load_vec<DT, V>(x + at, v);
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = act_f<ACT>(fmaf(v[j] - mu[j], a[j], b[j]), slope) * scale;
-            store_vec<DT, V>(y + at, v);
-        }
+        walk_apply<DT, V, ACT, true>(x, y, w, p, mu, a, b, slope, scale);
     }
+}
+
+// The place of a one-launch work-group: slab blockIdx.x (p.slab groups) of sample blockIdx.y; the walk covers all of its rows
+template <int V>
+__device__ __forceinline__ Walk slab_walk(const GnShape& p, int& g0, int& gs, int& width) {
+    g0 = (int)blockIdx.x * p.slab;
+    gs = p.groups - g0 < p.slab ? p.groups - g0 : p.slab;
+    width = gs * p.cg;
+    Walk w;
+    w.tx = (int)threadIdx.x % p.tile;
+    w.ty = (int)threadIdx.x / p.tile;
+    w.rp = p.rp;
+    w.row0 = (int64_t)blockIdx.y * p.l;
+    w.first = 0;
+    w.r_end = p.l;
+    w.c0 = g0 * p.cg + w.tx * V;
+    w.mine = w.ty < w.rp && w.tx * V < width;
+    return w;
+}
+
+template <int DT, int V, int ACT, bool KEEP>
+__global__ __launch_bounds__(kFused) void gn_fused_kernel(const typename Elem<DT>::T* __restrict__ x, const float* __restrict__ weight,
+                                                          const float* __restrict__ bias, typename Elem<DT>::T* __restrict__ y,
+                                                          float* __restrict__ mean, float* __restrict__ rstd, int8_t* __restrict__ codes,
+                                                          uint8_t* __restrict__ scales, float eps, float slope, float scale,
+                                                          const GnShape p) {
+    __shared__ double2 red[kFused];
+    __shared__ double2 unit[kFused];
+    __shared__ float2 stat[kFused];
+    int g0, gs, width;
+    const Walk w = slab_walk<V>(p, g0, gs, width);
+    const int tid = threadIdx.x;
+    const bool whole = p.cg % V == 0;
+    double sx[V], sxx[V];
+    walk_sums<DT, V, KEEP>(x, codes, scales, w, p, sx, sxx);
+    // unit sums of the slab: of its channel vectors, or of its channels (at most kFused of them: gn_slab)
+    const int rounds = whole ? 1 : V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (j >= rounds) break;
+        double2 t{sx[j], sxx[j]};
+        if (whole)
+#pragma unroll
+            for (int i = 1; i < V; ++i) { t.x += sx[i]; t.y += sxx[i]; }
+        __syncthreads();
+        red[tid] = t;
+        fold_rows(red, w.tx, w.ty, p.tile, p.rp, w.ty < p.rp);
+        if (w.ty == 0 && w.mine) unit[whole ? w.tx : w.tx * V + j] = red[w.tx];
+    }
+    __syncthreads();
+    const int per = whole ? p.cg / V : p.cg;
+    for (int g = tid; g < gs; g += (int)blockDim.x) {
+        double2 t = unit[g * per];
+        for (int u = 1; u < per; ++u) {
+            t.x += unit[g * per + u].x;
+            t.y += unit[g * per + u].y;
+        }
+        const float2 s = moments(t.x, t.y, (double)p.l * p.cg, eps);
+        stat[g] = s;
+        mean[(int64_t)blockIdx.y * p.groups + g0 + g] = s.x;
+        rstd[(int64_t)blockIdx.y * p.groups + g0 + g] = s.y;
+    }
+    __syncthreads();
+    if (!w.mine) return;
+    float mu[V], a[V], b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float2 s = stat[(w.tx * V + j) / p.cg];
+        mu[j] = s.x;
+        a[j] = s.y * (weight ? weight[w.c0 + j] : 1.0f) * Act<ACT>::kArg;
+        b[j] = (bias ? bias[w.c0 + j] : 0.0f) * Act<ACT>::kArg;
+    }
+    walk_apply<DT, V, ACT, false>(x, y, w, p, mu, a, b, slope, scale);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------------
 
-// V neighbours of the input: from the tensor, or (KEPT) what their codes stand for
+// kQ rows of the input: from the tensor, or (KEPT) from their codes
 template <int DT, int V, bool KEPT>
-__device__ __forceinline__ void load_input(const typename Elem<DT>::T* x, const int8_t* codes, const uint8_t* scales, int64_t row,
-                                           int c0, const GnShape& p, float (&v)[V]) {
-    if constexpr (KEPT) load_codes<V>(codes + row * p.blocks * kBlk8 + c0, block8_step(scales[(int64_t)(c0 / kBlk8) * p.rows + row]), v);
-    else load_vec<DT, V>(x + row * p.c + c0, v);
+struct Input {
+    Raw<DT, V> raw[kQ];
+    RawCodes<V> code[kQ];
+    unsigned e;
+    __device__ __forceinline__ void load(const typename Elem<DT>::T* x, const int8_t* codes, const uint8_t* scales, int64_t row, int c0,
+                                         int have, const GnShape& p) {
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int i = 0; i < kQ; ++i)
+                if (i < have) code[i].load(codes + (row + i) * p.blocks * kBlk8 + c0);
+            const uint8_t* from = scales + (int64_t)(c0 / kBlk8) * p.rows + row;
+            e = 0;
+            if (have == kQ) {
+                __builtin_memcpy(&e, from, 4);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kQ; ++i)
+                    if (i < have) e |= (unsigned)from[i] << (8 * i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kQ; ++i)
+                if (i < have) raw[i].load(x + (row + i) * p.c + c0);
+        }
+    }
+    __device__ __forceinline__ void get(int i, float (&v)[V]) const {
+        if constexpr (KEPT) code[i].get(block8_step((e >> (8 * i)) & 0xffu), v);
+        else raw[i].get(v);
+    }
+};
+
+// what a lane needs of its channels: the mean, and t = (x - mean) * a + b (b: from zero)
+template <int V>
+struct Affine {
+    float mu[V], a[V], b[V];
+};
+
+// a thread's sums over its rows of g = gy act'(z) and of g (x - mean)
+template <int DT, int V, int ACT, bool KEPT>
+__device__ __forceinline__ void walk_bwd_sums(const typename Elem<DT>::T* __restrict__ gy, const typename Elem<DT>::T* __restrict__ x,
+                                              const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const Walk& w,
+                                              const GnShape& p, const Affine<V>& f, float slope, float (&s1)[V], float (&s2)[V]) {
+    for (int64_t r = w.first + kQ * w.ty; r < w.r_end; r += kQ * w.rp) {
+        const int64_t row = w.row0 + r;
+        const int have = w.r_end - r < kQ ? (int)(w.r_end - r) : kQ;
+        Input<DT, V, KEPT> in;
+        Raw<DT, V> raw[kQ];
+        in.load(x, codes, scales, row, w.c0, have, p);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            if (i < have) raw[i].load(gy + (row + i) * p.c + w.c0);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            if (i < have) {
+                float v[V], g[V];
+                in.get(i, v);
+                raw[i].get(g);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float d = v[j] - f.mu[j];
+                    const float dz = g[j] * Act<ACT>::derivative(fmaf(d, f.a[j], f.b[j]), slope);
+                    s1[j] += dz;
+                    s2[j] = fmaf(dz, d, s2[j]);
+                }
+            }
+    }
 }
 
-// record [n][chunk][channel]: sum dz and sum dz xhat over the chunk's rows
+// gx = ga * g + (x - mean) * gd + ge, g as above
+template <int DT, int V, int ACT, bool KEPT, bool STREAM>
+__device__ __forceinline__ void walk_bwd_apply(const typename Elem<DT>::T* __restrict__ gy, const typename Elem<DT>::T* __restrict__ x,
+                                               const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                               typename Elem<DT>::T* __restrict__ gx, const Walk& w, const GnShape& p, const Affine<V>& f,
+                                               const float (&ga)[V], const float (&gd)[V], const float (&ge)[V], float slope) {
+    for (int64_t r = w.first + kQ * w.ty; r < w.r_end; r += kQ * w.rp) {
+        const int64_t row = w.row0 + r;
+        const int have = w.r_end - r < kQ ? (int)(w.r_end - r) : kQ;
+        Input<DT, V, KEPT> in;
+        Raw<DT, V> raw[kQ];
+        in.load(x, codes, scales, row, w.c0, have, p);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            if (i < have) raw[i].load(gy + (row + i) * p.c + w.c0);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            if (i < have) {
+                float v[V], g[V];
+                in.get(i, v);
+                raw[i].get(g);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float d = v[j] - f.mu[j];
+                    const float dz = g[j] * Act<ACT>::derivative(fmaf(d, f.a[j], f.b[j]), slope);
+                    v[j] = fmaf(ga[j], dz, fmaf(d, gd[j], ge[j]));
+                }
+                store_vec<DT, V, STREAM>(gx + (row + i) * p.c + w.c0, v);
+            }
+    }
+}
+
+// the four tensors every backward kernel reads besides gy
+struct BwdIn {
+    const float *mean, *rstd, *weight, *bias;
+};
+
+template <int V, int ACT>
+__device__ __forceinline__ void load_affine(const BwdIn& in, int64_t n, int c0, const GnShape& p, Affine<V>& f) {
+    int g[V];
+    groups_of<V>(c0, p.cg, g);
+    load_param<V>(in.weight, c0, 1.0f, f.a);
+    load_param<V>(in.bias, c0, 0.0f, f.b);
+    float mu = 0.0f, rs = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (j == 0 || g[j] != g[j - 1]) {
+            mu = in.mean[n * p.groups + g[j]];
+            rs = in.rstd[n * p.groups + g[j]];
+        }
+        f.mu[j] = mu;
+        f.a[j] *= rs * Act<ACT>::kArg;
+        f.b[j] *= Act<ACT>::kArg;
+    }
+}
+
+// record [n][chunk][channel]: the two sums over the chunk's rows
 template <int DT, int V, int ACT, bool KEPT>
 __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const typename Elem<DT>::T* __restrict__ gy,
                                                              const typename Elem<DT>::T* __restrict__ x,
                                                              const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                             const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                             const float* __restrict__ weight, const float* __restrict__ bias,
-                                                             float2* __restrict__ rec, float slope, float scale, const GnShape p) {
-    __shared__ float2 red[kBlock * V];
+                                                             const BwdIn in, float2* __restrict__ rec, float slope, const GnShape p) {
+    __shared__ float2 red[V][kBlock];
     const int n = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
-    const int tx = tid % p.tile, ty = tid / p.tile;
-    const int64_t r_begin = (int64_t)chunk * p.chunk_rows;
-    const int64_t r_end = r_begin + p.chunk_rows < p.l ? r_begin + p.chunk_rows : p.l;
+    Walk w;
+    w.tx = tid % p.tile;
+    w.ty = tid / p.tile;
+    w.rp = p.rp;
+    w.row0 = (int64_t)n * p.l;
+    w.first = (int64_t)chunk * p.chunk_rows;
+    w.r_end = w.first + p.chunk_rows < p.l ? w.first + p.chunk_rows : p.l;
     for (int lane0 = 0; lane0 < p.lanes; lane0 += p.tile) {
-        const int c0 = (lane0 + tx) * V;
+        w.c0 = (lane0 + w.tx) * V;
+        w.mine = w.ty < w.rp && w.c0 < p.c;
         float s1[V], s2[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
-        if (ty < p.rp && c0 < p.c) {
-            float mu[V], rs[V], w[V], b[V];
+        if (w.mine) {
+            Affine<V> f;
+            load_affine<V, ACT>(in, n, w.c0, p, f);
+            walk_bwd_sums<DT, V, ACT, KEPT>(gy, x, codes, scales, w, p, f, slope, s1, s2);
+        }
+        __syncthreads();
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const int64_t g = (int64_t)n * p.groups + (c0 + j) / p.cg;
-                mu[j] = mean[g];
-                rs[j] = rstd[g];
-                w[j] = weight ? weight[c0 + j] : 1.0f;
-                b[j] = bias ? bias[c0 + j] : 0.0f;
-            }
-            for (int64_t r = r_begin + ty; r < r_end; r += p.rp) {
-                const int64_t row = (int64_t)n * p.l + r;
-                float v[V], g[V];
-                load_input<DT, V, KEPT>(x, codes, scales, row, c0, p, v);
-                load_vec<DT, V>(gy + row * p.c + c0, g);
+        for (int j = 0; j < V; ++j) red[j][tid] = float2{s1[j], s2[j]};
+        int half = 1;
+        while (half < p.rp) half <<= 1;
+        for (half >>= 1; half >= 1; half >>= 1) {
+            __syncthreads();
+            if (w.ty < half && w.ty + half < p.rp)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float xh = (v[j] - mu[j]) * rs[j];
-                    const float dz = g[j] * (act_slope_f<ACT>(fmaf(xh, w[j], b[j]), slope) * scale);
-                    s1[j] += dz;
-                    s2[j] = fmaf(dz, xh, s2[j]);
+                    const float2 o = red[j][(w.ty + half) * p.tile + w.tx];
+                    red[j][tid].x += o.x;
+                    red[j][tid].y += o.y;
                 }
-            }
         }
-        __syncthreads();
+        if (w.ty == 0 && w.mine)
 #pragma unroll
-        for (int j = 0; j < V; ++j) red[tid * V + j] = float2{s1[j], s2[j]};
-        __syncthreads();
-        for (int u = tid; u < p.tile * V; u += kBlock) {
-            const int ch = lane0 * V + u;
-            if (ch >= p.c) continue;
-            float2 t = red[u];
-            for (int y = 1; y < p.rp; ++y) {
-                const float2 o = red[y * p.tile * V + u];
-                t.x += o.x;
-                t.y += o.y;
-            }
-            rec[((int64_t)n * p.chunks + chunk) * p.c + ch] = t;
-        }
+            for (int j = 0; j < V; ++j) rec[((int64_t)n * p.chunks + chunk) * p.c + w.c0 + j] = red[j][tid];
     }
 }
 
-// one work-group per (sample, group): the channels' totals and the group's two means
+// one work-group per (sample, group): the channels' totals {sum dz, sum dz xhat} and the group's two means
 __global__ __launch_bounds__(kBlock) void gn_bwd_totals_kernel(const float2* __restrict__ rec, const float* __restrict__ weight,
-                                                               float2* __restrict__ totals, float2* __restrict__ means,
-                                                               const GnShape p) {
+                                                               const float* __restrict__ rstd, float2* __restrict__ totals,
+                                                               float2* __restrict__ means, float scale, const GnShape p) {
     __shared__ double2 red[kBlock];
     const int g = blockIdx.x, n = blockIdx.y, tid = threadIdx.x;
     const int width = p.cg < kBlock ? p.cg : kBlock, depth = kBlock / width;
     const int tx = tid % width, ty = tid / width;
+    const double s1 = scale, s2 = (double)scale * rstd[(int64_t)n * p.groups + g];
     double m1 = 0.0, m2 = 0.0;
     for (int u0 = 0; u0 < p.cg; u0 += width) {
         const int ch = g * p.cg + u0 + tx;
-        const bool on = u0 + tx < p.cg;
+        const bool on = u0 + tx < p.cg && ty < depth;
         double a = 0.0, b = 0.0;
-        if (on && ty < depth)
+        if (on)
             for (int chunk = ty; chunk < p.chunks; chunk += depth) {
                 const float2 t = rec[((int64_t)n * p.chunks + chunk) * p.c + ch];
                 a += t.x;
                 b += t.y;
             }
         __syncthreads();
-        red[tid] = double2{a, b};
-        __syncthreads();
+        red[tid] = double2{a * s1, b * s2};
+        fold_rows(red, tx, ty, width, depth, ty < depth);
         if (on && ty == 0) {
-            for (int y = 1; y < depth; ++y) {
-                a += red[y * width + tx].x;
-                b += red[y * width + tx].y;
-            }
-            totals[(int64_t)n * p.c + ch] = float2{(float)a, (float)b};
+            const double2 t = red[tx];
+            totals[(int64_t)n * p.c + ch] = float2{(float)t.x, (float)t.y};
             const double w = weight ? weight[ch] : 1.0;
-            m1 += w * a;
-            m2 += w * b;
+            m1 += w * t.x;
+            m2 += w * t.y;
         }
     }
     __syncthreads();
     red[tid] = double2{m1, m2};
-    __syncthreads();
-    for (int half = kBlock / 2; half >= 1; half >>= 1) {
-        if (tid < half) {
-            red[tid].x += red[tid + half].x;
-            red[tid].y += red[tid + half].y;
-        }
-        __syncthreads();
-    }
+    fold_rows(red, 0, tid, 1, kBlock, true);
     if (tid == 0) {
         const double m = (double)p.l * p.cg;
         means[(int64_t)n * p.groups + g] = float2{(float)(red[0].x / m), (float)(red[0].y / m)};
@@ -317,11 +640,10 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_totals_kernel(const float2* __r
 }
 
 // gw, gb: the samples' channel totals added in order
-__global__ __launch_bounds__(kBlock) void gn_bwd_weight_kernel(const float2* __restrict__ totals, float* __restrict__ gw,
-                                                               float* __restrict__ gb, int n, int c) {
-    const int ch = blockIdx.x * kBlock + threadIdx.x;
-    if (ch >= c) return;
+__device__ __forceinline__ void weight_grads(const float2* __restrict__ totals, float* __restrict__ gw, float* __restrict__ gb, int n,
+                                             int c, int ch) {
     double a = 0.0, b = 0.0;
+#pragma unroll 8
     for (int i = 0; i < n; ++i) {
         const float2 t = totals[(int64_t)i * c + ch];
         a += t.x;
@@ -330,48 +652,127 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_weight_kernel(const float2* __r
     if (gb) gb[ch] = (float)a;
     if (gw) gw[ch] = (float)b;
 }
+__global__ __launch_bounds__(kBlock) void gn_bwd_weight_kernel(const float2* __restrict__ totals, float* __restrict__ gw,
+                                                               float* __restrict__ gb, int n, int c) {
+    const int ch = blockIdx.x * kBlock + threadIdx.x;
+    if (ch < c) weight_grads(totals, gw, gb, n, c, ch);
+}
+
+template <int V>
+__device__ __forceinline__ void bwd_factors(float rs, float2 m, float w, float scale, float& ga, float& gd, float& ge) {
+    ga = rs * w * scale;
+    gd = -rs * rs * m.y;
+    ge = -rs * m.x;
+}
 
 template <int DT, int V, int ACT, bool KEPT>
 __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const typename Elem<DT>::T* __restrict__ gy,
                                                               const typename Elem<DT>::T* __restrict__ x,
                                                               const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                              const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                              const float* __restrict__ weight, const float* __restrict__ bias,
-                                                              const float2* __restrict__ means, typename Elem<DT>::T* __restrict__ gx,
-                                                              float slope, float scale, const GnShape p) {
-    const int n = blockIdx.y, tid = threadIdx.x;
-    const int tx = tid % p.tile, ty = tid / p.tile;
-    const int64_t r_begin = (int64_t)blockIdx.x * p.chunk_rows;
-    const int64_t r_end = r_begin + p.chunk_rows < p.l ? r_begin + p.chunk_rows : p.l;
-    if (ty >= p.rp) return;
+                                                              const BwdIn in, const float2* __restrict__ means,
+                                                              const float2* __restrict__ totals, float* __restrict__ gw,
+                                                              float* __restrict__ gb, typename Elem<DT>::T* __restrict__ gx, float slope,
+                                                              float scale, const GnShape p) {
+    const int n = (int)gridDim.y - 1 - (int)blockIdx.y, chunk = (int)gridDim.x - 1 - (int)blockIdx.x, tid = threadIdx.x;
+    if (totals) {                                                  // gw and gb on the way, 256 channels a work-group
+        const int blocks = (int)(gridDim.x * gridDim.y);
+        for (int ch = (int)(blockIdx.y * gridDim.x + blockIdx.x) * kBlock + tid; ch < p.c; ch += blocks * kBlock)
+            weight_grads(totals, gw, gb, (int)gridDim.y, p.c, ch);
+    }
+    Walk w;
+    w.tx = tid % p.tile;
+    w.ty = tid / p.tile;
+    w.rp = p.rp;
+    w.row0 = (int64_t)n * p.l;
+    w.first = (int64_t)chunk * p.chunk_rows;
+    w.r_end = w.first + p.chunk_rows < p.l ? w.first + p.chunk_rows : p.l;
+    if (w.ty >= w.rp) return;
     for (int lane0 = 0; lane0 < p.lanes; lane0 += p.tile) {
-        const int c0 = (lane0 + tx) * V;
-        if (c0 >= p.c) return;
-        float mu[V], rs[V], w[V], b[V], m1[V], m2[V];
+        w.c0 = (lane0 + w.tx) * V;
+        if (w.c0 >= p.c) return;
+        Affine<V> f;
+        load_affine<V, ACT>(in, n, w.c0, p, f);
+        float ga[V], gd[V], ge[V];
+        int g[V];
+        groups_of<V>(w.c0, p.cg, g);
+        load_param<V>(in.weight, w.c0, 1.0f, ga);
+        float rs = 0.0f;
+        float2 m{0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int64_t g = (int64_t)n * p.groups + (c0 + j) / p.cg;
-            mu[j] = mean[g];
-            rs[j] = rstd[g];
-            w[j] = weight ? weight[c0 + j] : 1.0f;
-            b[j] = bias ? bias[c0 + j] : 0.0f;
-            m1[j] = means[g].x;
-            m2[j] = means[g].y;
+            if (j == 0 || g[j] != g[j - 1]) {
+                rs = in.rstd[(int64_t)n * p.groups + g[j]];
+                m = means[(int64_t)n * p.groups + g[j]];
+            }
+            bwd_factors<V>(rs, m, ga[j], scale, ga[j], gd[j], ge[j]);
         }
-        for (int64_t r = r_begin + ty; r < r_end; r += p.rp) {
-            const int64_t row = (int64_t)n * p.l + r;
-            float v[V], g[V];
-            load_input<DT, V, KEPT>(x, codes, scales, row, c0, p, v);
-            load_vec<DT, V>(gy + row * p.c + c0, g);
+        walk_bwd_apply<DT, V, ACT, KEPT, true>(gy, x, codes, scales, gx, w, p, f, ga, gd, ge, slope);
+    }
+}
+
+// one launch: a sample's slab of groups; totals [n][c] for the weights' kernel, or (one sample) gw and gb themselves
+template <int DT, int V, int ACT, bool KEPT>
+__global__ __launch_bounds__(kFused) void gn_bwd_fused_kernel(const typename Elem<DT>::T* __restrict__ gy,
+                                                              const typename Elem<DT>::T* __restrict__ x,
+                                                              const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                              const BwdIn in, float2* __restrict__ totals, float* __restrict__ gw,
+                                                              float* __restrict__ gb, typename Elem<DT>::T* __restrict__ gx, float slope,
+                                                              float scale, const GnShape p) {
+    __shared__ float2 red[V][kFused];
+    __shared__ float2 mean[kFused];
+    int g0, gs, width;
+    const Walk w = slab_walk<V>(p, g0, gs, width);
+    const int tid = threadIdx.x;
+    Affine<V> f;
+    float s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
+    if (w.mine) {
+        load_affine<V, ACT>(in, blockIdx.y, w.c0, p, f);
+        walk_bwd_sums<DT, V, ACT, KEPT>(gy, x, codes, scales, w, p, f, slope, s1, s2);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) red[j][tid] = float2{s1[j], s2[j]};
+    int half = 1;
+    while (half < p.rp) half <<= 1;
+    for (half >>= 1; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (w.ty < half && w.ty + half < p.rp)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xh = (v[j] - mu[j]) * rs[j];
-                const float dz = g[j] * (act_slope_f<ACT>(fmaf(xh, w[j], b[j]), slope) * scale);
-                v[j] = rs[j] * (fmaf(w[j], dz, -m1[j]) - xh * m2[j]);
+                const float2 o = red[j][(w.ty + half) * p.tile + w.tx];
+                red[j][tid].x += o.x;
+                red[j][tid].y += o.y;
             }
-            store_vec<DT, V>(gx + row * p.c + c0, v);
-        }
     }
+    __syncthreads();
+    for (int i = tid; i < gs; i += (int)blockDim.x) {              // the group's channels in order
+        const int64_t g = (int64_t)blockIdx.y * p.groups + g0 + i;
+        const double k1 = scale, k2 = (double)scale * in.rstd[g];
+        double m1 = 0.0, m2 = 0.0;
+        for (int u = i * p.cg; u < (i + 1) * p.cg; ++u) {
+            const float2 t = red[u % V][u / V];
+            const int ch = g0 * p.cg + u;
+            const double w1 = in.weight ? in.weight[ch] : 1.0, a = t.x * k1, b = t.y * k2;
+            m1 += w1 * a;
+            m2 += w1 * b;
+            if (totals) totals[(int64_t)blockIdx.y * p.c + ch] = float2{(float)a, (float)b};
+            if (gb) gb[ch] = (float)a;
+            if (gw) gw[ch] = (float)b;
+        }
+        const double m = (double)p.l * p.cg;
+        mean[i] = float2{(float)(m1 / m), (float)(m2 / m)};
+    }
+    __syncthreads();
+    if (!w.mine || !gx) return;
+    float ga[V], gd[V], ge[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int g = (w.tx * V + j) / p.cg;
+        bwd_factors<V>(in.rstd[(int64_t)blockIdx.y * p.groups + g0 + g], mean[g], in.weight ? in.weight[w.c0 + j] : 1.0f, scale, ga[j],
+                       gd[j], ge[j]);
+    }
+    walk_bwd_apply<DT, V, ACT, KEPT, false>(gy, x, codes, scales, gx, w, p, f, ga, gd, ge, slope);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
@@ -383,7 +784,19 @@ bool gn_shape_ok(int64_t n, int64_t l, int64_t c, int64_t groups) {
            c % groups == 0 && l <= ((int64_t)1 << 40) / c;
 }
 
-GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int v) {
+// Groups of a one-launch work-group: whole vectors, whole 8-bit blocks where it writes them (or the whole row), at least 64 bytes of a
+// row (one group's share is often less, and every 64-byte piece is read whole); 0 if there is no such slab.
+int gn_slab(int64_t c, int64_t groups, int v, int esize, bool keep) {
+    const int64_t cg = c / groups;
+    for (int64_t s = 1; s <= groups; ++s) {
+        const int64_t w = s * cg;
+        if (w > kFused || s > kFused) return 0;                    // a lane, a unit and a group at most for each thread
+        if (s == groups || (w % v == 0 && (!keep || w % kBlk8 == 0) && w * esize >= 64)) return (int)s;
+    }
+    return 0;
+}
+
+GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int v, int esize, bool keep) {
     GnShape p;
     p.l = l;
     p.rows = n * l;
@@ -391,19 +804,41 @@ GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int v) {
     p.groups = (int)groups;
     p.cg = (int)(c / groups);
     p.blocks = (int)ceil_div64(c, kBlk8);
+    p.units = p.cg % v == 0 ? (int)c / v : (int)c;
+    p.slab = gn_slab(c, groups, v, esize, keep);
+    p.slabs = p.slab ? (int)ceil_div64(groups, p.slab) : 0;
+    // One launch where a thread of kFused makes at most 8 / kQ trips over its slab, twice; 16 where the whole tensor is so small (4 MB)
+    // that launches are what costs.  (knob 0, for tests: never)
+    if (p.slab) {
+        const int64_t trips = ceil_div64(l * p.slab * p.cg, (int64_t)kFused * v) * tuning_knob("SAE_GN_ONE_LAUNCH", 1);
+        if (trips == 0 || trips > (n * l * c * esize <= ((int64_t)4 << 20) ? 16 : 8)) p.slab = 0;
+    }
+    if (p.slab) {
+        p.lanes = (int)ceil_div64((int64_t)p.slab * p.cg, kBlk8) * (kBlk8 / v);
+        p.tile = p.lanes;
+        p.rp = kFused / p.tile;
+        while (p.rp > 1 && (int64_t)(p.rp / 2) * kQ >= l) p.rp /= 2;          // (no more threads than rows)
+        p.chunk_rows = 0;
+        p.chunks = 1;
+        return p;
+    }
     p.lanes = p.blocks * (kBlk8 / v);
     p.tile = p.lanes < kBlock ? p.lanes : kBlock;
     p.rp = kBlock / p.tile;
-    // ~8 work-groups per CU over the whole batch, at least four rows for each thread
-    const int64_t most = ceil_div64(l, 4 * (int64_t)p.rp), want = ceil_div64(2048, n > 0 ? n : 1);
-    const int64_t chunks = most < want ? most : want;
-    p.chunk_rows = (int)(ceil_div64(ceil_div64(l, chunks > 0 ? chunks : 1), p.rp) * p.rp);
+    // Up to 8 work-groups per CU over the whole batch, while each thread has four trips of kQ rows (one trip alone is all prologue:
+    // [16, 256, 64, 64] bf16 took 36 us so); down to 2 per CU with fewer trips than that.
+    const int64_t step = (int64_t)kQ * p.rp, each = n > 0 ? n : 1;
+    int64_t chunks = ceil_div64(l, 4 * step);
+    if (chunks > ceil_div64(2048, each)) chunks = ceil_div64(2048, each);
+    if (chunks < ceil_div64(512, each)) chunks = ceil_div64(512, each);
+    if (chunks > ceil_div64(l, step)) chunks = ceil_div64(l, step);
+    p.chunk_rows = (int)(ceil_div64(ceil_div64(l, chunks > 0 ? chunks : 1), step) * step);
     p.chunks = (int)ceil_div64(l, p.chunk_rows > 0 ? p.chunk_rows : 1);
-    p.units = p.cg % v == 0 ? (int)c / v : (int)c;
     return p;
 }
 
 int64_t gn_workspace(const GnShape& p, int64_t n, bool backward) {
+    if (p.slab) return backward && n > 1 ? n * p.c * (int64_t)sizeof(float2) : 0;
     if (!backward) return n * p.chunks * p.units * (int64_t)sizeof(double2);
     return (n * p.chunks * (int64_t)p.c + n * p.c + n * p.groups) * (int64_t)sizeof(float2);
 }
@@ -423,78 +858,105 @@ struct GnArgs {
     hipStream_t stream;
 };
 
-template <int DT, int V>
-int gn_forward(const GnArgs& a, const GnShape& p) {
+template <int DT, int V, int ACT>
+void gn_forward_as(const GnArgs& a, const GnShape& p) {
     using T = typename Elem<DT>::T;
+    if (p.slab) {
+        const dim3 grid((unsigned)p.slabs, (unsigned)a.n), block((unsigned)(p.tile * p.rp));
+        if (a.codes)
+            hipLaunchKernelGGL((gn_fused_kernel<DT, V, ACT, true>), grid, block, 0, a.stream, (const T*)a.x, a.weight, a.bias, (T*)a.out,
+                               a.mean, a.rstd, a.codes, a.scales, a.eps, a.slope, a.scale, p);
+        else
+            hipLaunchKernelGGL((gn_fused_kernel<DT, V, ACT, false>), grid, block, 0, a.stream, (const T*)a.x, a.weight, a.bias,
+                               (T*)a.out, a.mean, a.rstd, a.codes, a.scales, a.eps, a.slope, a.scale, p);
+        return;
+    }
     const dim3 grid((unsigned)p.chunks, (unsigned)a.n), block(kBlock);
     double2* rec = (double2*)a.ws;
     if (a.codes)
         hipLaunchKernelGGL((gn_sums_kernel<DT, V, true>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
     else
         hipLaunchKernelGGL((gn_sums_kernel<DT, V, false>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
+    if (p.groups <= kFoldGroups && p.chunks * p.units <= kFoldRecords) {
+        hipLaunchKernelGGL((gn_apply_kernel<DT, V, ACT, true>), grid, block, 0, a.stream, (const T*)a.x, (const double2*)rec, a.mean,
+                           a.rstd, a.weight, a.bias, (T*)a.out, a.eps, a.slope, a.scale, p);
+        return;
+    }
     hipLaunchKernelGGL(gn_totals_kernel, dim3((unsigned)p.groups, (unsigned)a.n), dim3(kWave), 0, a.stream, (const double2*)rec,
                        a.mean, a.rstd, a.eps, p);
-#define SAE_GN_APPLY(ACT)                                                                                                      \
-    hipLaunchKernelGGL((gn_apply_kernel<DT, V, ACT>), grid, block, 0, a.stream, (const T*)a.x, (const float*)a.mean,           \
-                       (const float*)a.rstd, a.weight, a.bias, (T*)a.out, a.slope, a.scale, p)
-    if (a.act == SAE_ACT_LRELU) SAE_GN_APPLY(SAE_ACT_LRELU);
-    else if (a.act == SAE_ACT_SILU) SAE_GN_APPLY(SAE_ACT_SILU);
-    else SAE_GN_APPLY(SAE_ACT_NONE);
-#undef SAE_GN_APPLY
-    return check_launch("sae_group_norm_act");
+    hipLaunchKernelGGL((gn_apply_kernel<DT, V, ACT, false>), grid, block, 0, a.stream, (const T*)a.x, (const double2*)rec, a.mean,
+                       a.rstd, a.weight, a.bias, (T*)a.out, a.eps, a.slope, a.scale, p);
 }
 
 template <int DT, int V, int ACT, bool KEPT>
-int gn_backward_as(const GnArgs& a, const GnShape& p) {
+void gn_backward_as(const GnArgs& a, const GnShape& p) {
     using T = typename Elem<DT>::T;
+    const BwdIn in{a.mean, a.rstd, a.weight, a.bias};
+    const bool weights = a.gw || a.gb;
+    if (p.slab) {
+        const dim3 grid((unsigned)p.slabs, (unsigned)a.n), block((unsigned)(p.tile * p.rp));
+        float2* totals = a.n > 1 && weights ? (float2*)a.ws : nullptr;
+        hipLaunchKernelGGL((gn_bwd_fused_kernel<DT, V, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
+                           (const int8_t*)a.codes, (const uint8_t*)a.scales, in, totals, totals ? nullptr : a.gw,
+                           totals ? nullptr : a.gb, (T*)a.out, a.slope, a.scale, p);
+        if (totals)
+            hipLaunchKernelGGL(gn_bwd_weight_kernel, dim3((unsigned)ceil_div(p.c, kBlock)), dim3(kBlock), 0, a.stream,
+                               (const float2*)totals, a.gw, a.gb, (int)a.n, p.c);
+        return;
+    }
     const dim3 grid((unsigned)p.chunks, (unsigned)a.n), block(kBlock);
     float2* rec = (float2*)a.ws;
     float2* totals = rec + a.n * p.chunks * (int64_t)p.c;
     float2* means = totals + a.n * p.c;
     hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, V, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
-                       (const int8_t*)a.codes, (const uint8_t*)a.scales, (const float*)a.mean, (const float*)a.rstd, a.weight,
-                       a.bias, rec, a.slope, a.scale, p);
+                       (const int8_t*)a.codes, (const uint8_t*)a.scales, in, rec, a.slope, p);
     hipLaunchKernelGGL(gn_bwd_totals_kernel, dim3((unsigned)p.groups, (unsigned)a.n), block, 0, a.stream, (const float2*)rec,
-                       a.weight, totals, means, p);
-    if (a.gw || a.gb)
-        hipLaunchKernelGGL(gn_bwd_weight_kernel, dim3((unsigned)ceil_div(p.c, kBlock)), block, 0, a.stream, (const float2*)totals,
-                           a.gw, a.gb, (int)a.n, p.c);
+                       a.weight, (const float*)a.rstd, totals, means, a.scale, p);
     if (a.out)
         hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
-                           (const int8_t*)a.codes, (const uint8_t*)a.scales, (const float*)a.mean, (const float*)a.rstd, a.weight,
-                           a.bias, (const float2*)means, (T*)a.out, a.slope, a.scale, p);
-    return check_launch("sae_group_norm_act_bwd");
-}
-
-template <int DT, int V, bool KEPT>
-int gn_backward(const GnArgs& a, const GnShape& p) {
-    if (a.act == SAE_ACT_LRELU) return gn_backward_as<DT, V, SAE_ACT_LRELU, KEPT>(a, p);
-    if (a.act == SAE_ACT_SILU) return gn_backward_as<DT, V, SAE_ACT_SILU, KEPT>(a, p);
-    return gn_backward_as<DT, V, SAE_ACT_NONE, KEPT>(a, p);
+                           (const int8_t*)a.codes, (const uint8_t*)a.scales, in, (const float2*)means,
+                           weights ? (const float2*)totals : (const float2*)nullptr, a.gw, a.gb, (T*)a.out, a.slope, a.scale, p);
+    else
+        hipLaunchKernelGGL(gn_bwd_weight_kernel, dim3((unsigned)ceil_div(p.c, kBlock)), block, 0, a.stream, (const float2*)totals,
+                           a.gw, a.gb, (int)a.n, p.c);
 }
 
 // V channels per lane in 16-byte accesses where the rows allow it, one channel where not
 bool gn_vector(int64_t c, int32_t dtype) { return c % (16 / elem_bytes(dtype)) == 0; }
 
+template <int DT, int V, int ACT>
+void gn_run(const GnArgs& a, const GnShape& p, bool backward) {
+    if (!backward) gn_forward_as<DT, V, ACT>(a, p);
+    else if (a.codes) gn_backward_as<DT, V, ACT, true>(a, p);
+    else gn_backward_as<DT, V, ACT, false>(a, p);
+}
+
+template <int DT, int V>
+void gn_run(const GnArgs& a, const GnShape& p, bool backward) {
+    if (a.act == SAE_ACT_LRELU) gn_run<DT, V, SAE_ACT_LRELU>(a, p, backward);
+    else if (a.act == SAE_ACT_SILU) gn_run<DT, V, SAE_ACT_SILU>(a, p, backward);
+    else gn_run<DT, V, SAE_ACT_NONE>(a, p, backward);
+}
+
 template <int DT>
-int gn_run(const GnArgs& a, const GnShape& p, bool vec, bool backward) {
-    if (!backward) return vec ? gn_forward<DT, Elem<DT>::kVec>(a, p) : gn_forward<DT, 1>(a, p);
-    if (a.codes) return vec ? gn_backward<DT, Elem<DT>::kVec, true>(a, p) : gn_backward<DT, 1, true>(a, p);
-    return vec ? gn_backward<DT, Elem<DT>::kVec, false>(a, p) : gn_backward<DT, 1, false>(a, p);
+void gn_run(const GnArgs& a, const GnShape& p, bool vec, bool backward) {
+    if (vec) gn_run<DT, Elem<DT>::kVec>(a, p, backward);
+    else gn_run<DT, 1>(a, p, backward);
 }
 
 int gn_dispatch(const char* what, GnArgs& a, int64_t l, int64_t c, int64_t groups, int32_t dtype, int64_t ws_bytes, bool backward) {
     const bool vec = gn_vector(c, dtype);
-    const GnShape p = gn_plan(a.n, l, c, groups, vec ? 16 / elem_bytes(dtype) : 1);
+    const GnShape p = gn_plan(a.n, l, c, groups, vec ? 16 / elem_bytes(dtype) : 1, elem_bytes(dtype), !backward && a.codes);
     const int64_t need = gn_workspace(p, a.n, backward);
-    if (!a.ws || ws_bytes < need)
+    if (need > 0 && (!a.ws || ws_bytes < need))
         return fail(SAE_EWORKSPACE, "%s: workspace %lld < %lld bytes (sae_group_norm_act_workspace)", what, (long long)ws_bytes,
                     (long long)need);
     for (const void* t : {a.gy, a.x, (const void*)a.out, (const void*)a.ws, (const void*)a.codes})
         if (!aligned16(t)) return fail(SAE_EINVAL, "%s: tensors must be 16-byte aligned", what);
-    if (dtype == SAE_F32) return gn_run<SAE_F32>(a, p, vec, backward);
-    if (dtype == SAE_BF16) return gn_run<SAE_BF16>(a, p, vec, backward);
-    return gn_run<SAE_F16>(a, p, vec, backward);
+    if (dtype == SAE_F32) gn_run<SAE_F32>(a, p, vec, backward);
+    else if (dtype == SAE_BF16) gn_run<SAE_BF16>(a, p, vec, backward);
+    else gn_run<SAE_F16>(a, p, vec, backward);
+    return check_launch(what);
 }
 
 }  // namespace
@@ -504,7 +966,9 @@ using namespace sae;
 
 extern "C" int64_t sae_group_norm_act_workspace(int64_t n, int64_t l, int64_t c, int64_t groups, int32_t dtype, int32_t backward) {
     if (!gn_shape_ok(n, l, c, groups) || !elem_known(dtype) || n == 0 || l == 0) return 0;
-    return gn_workspace(gn_plan(n, l, c, groups, gn_vector(c, dtype) ? 16 / elem_bytes(dtype) : 1), n, backward != 0);
+    // (a forward pass that keeps its input has the wider slabs, and is in one launch only where one that does not is too)
+    return gn_workspace(gn_plan(n, l, c, groups, gn_vector(c, dtype) ? 16 / elem_bytes(dtype) : 1, elem_bytes(dtype), !backward), n,
+                        backward != 0);
 }
 
 extern "C" int sae_group_norm_act(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,

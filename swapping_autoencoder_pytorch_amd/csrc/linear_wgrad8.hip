@@ -31,7 +31,6 @@ namespace {
 constexpr int kBN = 128;       // channels of x of a tile
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 template <int DT>
 __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {

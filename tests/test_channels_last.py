@@ -48,14 +48,16 @@ def test_refusals(emu_lib):
             ops.Checkpoint8(*good, shape=(3, 40))
 
 
-def test_entry_points_refuse(emu_lib):
+def test_entry_points_refuse(emu_lib, monkeypatch):
     """the C entry points' own checks: null tensors, unknown codes, misalignment, short workspaces"""
+    monkeypatch.setenv("SAE_GN_ONE_LAUNCH", "0")     # the form that needs a workspace
     x = torch.randn(4, 16)
     y, w = torch.empty_like(x), torch.ones(16)
     stats = torch.empty(2, 8)
     codes, scales = torch.empty(4, 32, dtype=torch.int8), torch.empty(1, 4, dtype=torch.uint8)
     n = emu_lib.query("group_norm_act_workspace", 2, 2, 16, 4, 0, 0)
     nb = emu_lib.query("group_norm_act_workspace", 2, 2, 16, 4, 0, 1)
+    assert n > 0 and nb > 0
     ws = torch.empty(max(n, nb), dtype=torch.uint8)
     p = lambda t: t.data_ptr()
     good = [p(x), p(w), p(w), p(y), p(stats[0]), p(stats[1]), p(codes), p(scales), 2, 2, 16, 4, 1e-5, 1, 0.2, 1.0, 0, p(ws), n, None]
@@ -163,6 +165,16 @@ def test_norm_emulated(emu_lib, dtype, shape):
         for i, act in enumerate(ACTS):
             K.check_norm("cpu", K.TYPES[dtype], shape, act, checkpoint=False, affine=i != 0)
             K.check_norm("cpu", K.TYPES[dtype], shape, act, checkpoint=True, affine=i != 1)
+
+
+@pytest.mark.parametrize("shape", K.NORM_SHAPES, ids=norm_id)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_in_three_launches_emulated(emu_lib, dtype, shape, monkeypatch):
+    """small groups through the kernels of the large ones (the knob exists in tuning builds only)"""
+    monkeypatch.setenv("SAE_GN_ONE_LAUNCH", "0")
+    with backend(emu_lib):
+        K.check_norm("cpu", K.TYPES[dtype], shape, "silu", checkpoint=False)
+        K.check_norm("cpu", K.TYPES[dtype], shape, "lrelu", checkpoint=True)
 
 
 @pytest.mark.parametrize("shape", K.WGRAD_SHAPES, ids=lambda s: "r%d_c%d_o%d" % s)
