@@ -11,82 +11,123 @@
 namespace sae {
 namespace {
 
-// One thread per V neighbours of a row padded to whole blocks; a block's LB = 32 / V lanes lie in one wave and meet in shuffles.
-template <int DT, int V>
+constexpr int kQ = 4;              // rows a thread takes: four loads under way, and the exponents of a block's four rows are a word
+
+struct PackShape {
+    int64_t rows, c, blocks;
+    int64_t lanes;             // channel vectors of a row padded to whole blocks
+    int tile, rp;              // of a work-group: lanes at a time, threads / tile (rows at a time: kQ of each)
+    int64_t tiles, chunks;     // of a row, of the rows
+};
+
+// A work-group takes one (chunk of rows, tile of lanes) after the other in strides of the grid.  ANY: rows that start anywhere and end
+// inside a vector.
+template <int DT, bool ANY>
 __global__ __launch_bounds__(kBlock) void checkpoint8_pack_kernel(const typename Elem<DT>::T* __restrict__ x,
                                                                   int8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                                  int64_t rows, int64_t c, int64_t blocks) {
-    constexpr int LB = kBlk8 / V;
-    const int64_t stride = (int64_t)gridDim.x * (kBlock / LB);
-    for (int64_t base = (int64_t)blockIdx.x * (kBlock / LB); base < rows * blocks; base += stride) {
-        const int64_t block = base + threadIdx.x / LB;
-        const bool live = block < rows * blocks;      // (whole groups of LB lanes are live or not)
-        const int64_t row = live ? block / blocks : 0, cb = live ? block - row * blocks : 0;
-        const int64_t col = cb * kBlk8 + (int64_t)(threadIdx.x % LB) * V;
-        Raw<DT, V> raw;
-        raw.zero();
-        if (live && col < c) raw.load(x + row * c + col);
-        const unsigned e = block8_exponent<DT>(block8_amax<LB>(raw.amax()));
-        if (!live) continue;
-        float v[V];
-        raw.get(v);
-        store_codes<V>(codes + row * blocks * kBlk8 + col, v, block8_inverse(e));
-        if (threadIdx.x % LB == 0) scales[cb * rows + row] = (uint8_t)e;
+                                                                  const PackShape p) {
+    constexpr int V = Elem<DT>::kVec, LB = kBlk8 / V;
+    const int tx = (int)threadIdx.x % p.tile, ty = (int)threadIdx.x / p.tile;
+    for (int64_t id = blockIdx.x; id < p.tiles * p.chunks; id += gridDim.x) {
+        const int64_t chunk = id / p.tiles, lane = (id - chunk * p.tiles) * p.tile + tx, c0 = lane * V;
+        const int64_t r = (chunk * p.rp + ty) * kQ;
+        const int have = ty >= p.rp || lane >= p.lanes || r >= p.rows ? 0 : p.rows - r < kQ ? (int)(p.rows - r) : kQ;
+        const int n = p.c - c0 < V ? (int)(p.c - c0) : V;           // (not positive in a row's padding)
+        Raw<DT> raw[kQ];
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {
+            raw[i].zero();
+            if (i < have && n > 0) {
+                if constexpr (ANY) raw[i].load_some(x + (r + i) * p.c + c0, n, p.c >= V);
+                else raw[i].load(x + (r + i) * p.c + c0);
+            }
+        }
+        unsigned word = 0;
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {                              // (whole blocks of lanes have the same rows)
+            const unsigned e = block8_exponent<DT>(block8_amax<LB>(raw[i].amax()));
+            word |= e << (8 * i);
+            if (i < have) {
+                float v[V];
+                raw[i].get(v);
+                store_codes<V>(codes + (r + i) * p.blocks * kBlk8 + c0, v, block8_inverse(e));
+            }
+        }
+        if (have > 0 && lane % LB == 0) store_exponents(scales + c0 / kBlk8 * p.rows + r, word, have);
     }
 }
 
-template <int DT, int V>
+template <int DT, bool ANY, bool STREAM>
 __global__ __launch_bounds__(kBlock) void checkpoint8_unpack_kernel(const int8_t* __restrict__ codes,
                                                                     const uint8_t* __restrict__ scales,
-                                                                    typename Elem<DT>::T* __restrict__ x, int64_t rows,
-                                                                    int64_t c, int64_t blocks) {
-    constexpr int LB = kBlk8 / V;
-    const int64_t stride = (int64_t)gridDim.x * (kBlock / LB);
-    for (int64_t block = (int64_t)blockIdx.x * (kBlock / LB) + threadIdx.x / LB; block < rows * blocks; block += stride) {
-        const int64_t row = block / blocks, cb = block - row * blocks;
-        const int64_t col = cb * kBlk8 + (int64_t)(threadIdx.x % LB) * V;
-        if (col >= c) continue;
-        RawCodes<V> raw;
-        raw.load(codes + row * blocks * kBlk8 + col);
-        float v[V];
-        raw.get(block8_step(scales[cb * rows + row]), v);
-        store_vec<DT, V>(x + row * c + col, v);
+                                                                    typename Elem<DT>::T* __restrict__ x, const PackShape p) {
+    constexpr int V = Elem<DT>::kVec;
+    const int tx = (int)threadIdx.x % p.tile, ty = (int)threadIdx.x / p.tile;
+    if (ty >= p.rp) return;
+    for (int64_t id = blockIdx.x; id < p.tiles * p.chunks; id += gridDim.x) {
+        const int64_t chunk = id / p.tiles, lane = (id - chunk * p.tiles) * p.tile + tx, c0 = lane * V;
+        const int64_t r = (chunk * p.rp + ty) * kQ;
+        if (c0 >= p.c || r >= p.rows) continue;
+        const int have = p.rows - r < kQ ? (int)(p.rows - r) : kQ, n = p.c - c0 < V ? (int)(p.c - c0) : V;
+        RawCodes<V> code[kQ];
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            if (i < have) code[i].load(codes + (r + i) * p.blocks * kBlk8 + c0);
+        const unsigned word = load_exponents(scales + c0 / kBlk8 * p.rows + r, have);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            if (i < have) {
+                float v[V];
+                code[i].get(block8_step((word >> (8 * i)) & 0xffu), v);
+                Raw<DT> raw;
+                raw.set(v);
+                if constexpr (ANY) raw.store_some(x + (r + i) * p.c + c0, n);
+                else raw.template store<STREAM>(x + (r + i) * p.c + c0);
+            }
     }
 }
 
-// work-groups of the two kernels, which walk what is behind them in strides of the grid (a launch holds 2^32 threads at most)
-unsigned checkpoint8_grid(int64_t rows, int64_t blocks, int lanes) {
-    const int64_t g = ceil_div64(rows * blocks, kBlock / lanes);
-    return (unsigned)(g > (1 << 20) ? 1 << 20 : g);
+PackShape pack_plan(int64_t rows, int64_t c, int v) {
+    PackShape p;
+    const int lb = kBlk8 / v;
+    p.rows = rows;
+    p.c = c;
+    p.blocks = ceil_div64(c, kBlk8);
+    p.lanes = p.blocks * lb;
+    const int64_t tiles = ceil_div64(p.lanes, kBlock);
+    p.tile = (int)(ceil_div64(ceil_div64(p.lanes, tiles), lb) * lb);       // tiles of even width, of whole blocks
+    p.tiles = ceil_div64(p.lanes, p.tile);
+    p.rp = kBlock / p.tile;
+    p.chunks = ceil_div64(rows, (int64_t)p.rp * kQ);
+    return p;
+}
+dim3 pack_grid(const PackShape& p) {
+    const int64_t g = p.tiles * p.chunks;                                   // (a launch holds 2^32 threads at most)
+    return dim3((unsigned)(g > (1 << 20) ? 1 << 20 : g));
 }
 
 template <int DT>
 int pack(const void* x, int8_t* codes, uint8_t* scales, int64_t rows, int64_t c, hipStream_t s) {
     using T = typename Elem<DT>::T;
-    const int64_t blocks = ceil_div64(c, kBlk8);
-    const bool vec = c % Elem<DT>::kVec == 0 && aligned16(x);
-    const unsigned g = checkpoint8_grid(rows, blocks, vec ? kBlk8 / Elem<DT>::kVec : kBlk8);
-    if (vec)
-        hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, Elem<DT>::kVec>), dim3(g), dim3(kBlock), 0, s, (const T*)x, codes,
-                           scales, rows, c, blocks);
+    const PackShape p = pack_plan(rows, c, Elem<DT>::kVec);
+    if (c % Elem<DT>::kVec == 0 && aligned16(x))
+        hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, false>), pack_grid(p), dim3(kBlock), 0, s, (const T*)x, codes, scales, p);
     else
-        hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, 1>), dim3(g), dim3(kBlock), 0, s, (const T*)x, codes, scales, rows,
-                           c, blocks);
+        hipLaunchKernelGGL((checkpoint8_pack_kernel<DT, true>), pack_grid(p), dim3(kBlock), 0, s, (const T*)x, codes, scales, p);
     return check_launch("sae_checkpoint8_pack");
 }
 
 template <int DT>
 int unpack(const int8_t* codes, const uint8_t* scales, void* x, int64_t rows, int64_t c, hipStream_t s) {
     using T = typename Elem<DT>::T;
-    const int64_t blocks = ceil_div64(c, kBlk8);
-    const bool vec = c % Elem<DT>::kVec == 0 && aligned16(x);
-    const unsigned g = checkpoint8_grid(rows, blocks, vec ? kBlk8 / Elem<DT>::kVec : kBlk8);
-    if (vec)
-        hipLaunchKernelGGL((checkpoint8_unpack_kernel<DT, Elem<DT>::kVec>), dim3(g), dim3(kBlock), 0, s, codes, scales,
-                           (T*)x, rows, c, blocks);
+    const PackShape p = pack_plan(rows, c, Elem<DT>::kVec);
+    const bool whole = c % Elem<DT>::kVec == 0 && aligned16(x), stream = rows * c * (int64_t)sizeof(T) > ((int64_t)32 << 20);   // > the L2s
+    if (whole && stream)
+        hipLaunchKernelGGL((checkpoint8_unpack_kernel<DT, false, true>), pack_grid(p), dim3(kBlock), 0, s, codes, scales, (T*)x, p);
+    else if (whole)
+        hipLaunchKernelGGL((checkpoint8_unpack_kernel<DT, false, false>), pack_grid(p), dim3(kBlock), 0, s, codes, scales, (T*)x, p);
     else
-        hipLaunchKernelGGL((checkpoint8_unpack_kernel<DT, 1>), dim3(g), dim3(kBlock), 0, s, codes, scales, (T*)x, rows, c,
-                           blocks);
+        hipLaunchKernelGGL((checkpoint8_unpack_kernel<DT, true, false>), pack_grid(p), dim3(kBlock), 0, s, codes, scales, (T*)x, p);
     return check_launch("sae_checkpoint8_unpack");
 }
 

@@ -14,7 +14,7 @@
 // or, where a sample's groups are small, all of it in one work-group per (sample, slab of whole groups): one launch.
 //
 // Layout of a walk: a lane owns V neighbouring channels (16 bytes) and takes four rows at a time, so that four loads are under way
-// and the exponents of four rows are one word.
+// and the exponents of four rows are one word.  ANY: rows (or slabs of them) that start anywhere and end inside a vector.
 //
 // Numerics: a thread adds x - x0 and (x - x0)^2 over its rows, x0 the first value it meets in the channel: at most the number of
 // its rows times the rounding of a plain sum, whatever the channel's mean.  The records are moments about zero in 64 bits, which
@@ -31,13 +31,14 @@ struct GnShape {
     int64_t l;                 // positions of a sample
     int64_t rows;              // n * l: rows of codes, stride of a block's exponents
     int c, groups, cg;
-    int lanes;                 // channel vectors of a row (of a slab), padded to whole 8-bit blocks
+    int lanes;                 // channel vectors of a row (of a slab); padded to whole 8-bit blocks where codes are written
     int tile;                  // lanes a work-group covers at a time
     int rp;                    // rows it covers at a time: threads / tile, kQ of each
     int chunk_rows;            // rows of a work-group
     int chunks;                // chunks of a sample
     int units;                 // records of a chunk: channel vectors if a vector lies in one group, channels if not
     int blocks;                // 8-bit blocks of a row
+    bool any;                  // vectors that start anywhere or end inside
     int slab, slabs;           // groups of a one-launch work-group (0: not that form), slabs of a sample
 };
 
@@ -73,31 +74,52 @@ struct Act {
 
 // The groups of a lane's V channels, one division for all of them
 template <int V>
-__device__ __forceinline__ void groups_of(int c0, int cg, int (&g)[V]) {
+__device__ __forceinline__ void groups_of(int c0, int cg, int most, int (&g)[V]) {
     int at = c0 / cg, left = cg - (c0 - at * cg);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        g[j] = at;
+        g[j] = at < most ? at : most - 1;                          // (behind the row's end: any that is there)
         if (--left == 0) { ++at; left = cg; }
     }
 }
 
 // V neighbours of a parameter (absent: all `none`)
 template <int V>
-__device__ __forceinline__ void load_param(const float* __restrict__ w, int c0, float none, float (&v)[V]) {
+__device__ __forceinline__ void load_param(const float* __restrict__ w, int c0, int n, float none, float (&v)[V]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = none;
     if (!w) return;
-    if constexpr (V >= 4) __builtin_memcpy(v, w + c0, sizeof(v));
-    else v[0] = w[c0];
+    if (n >= V) {
+        __builtin_memcpy(v, w + c0, sizeof(v));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < V - 1; ++j)
+        if (j < n) v[j] = w[c0 + j];
 }
 
 // Where a thread stands in a walk over rows [r_begin, r_end) of sample n
 struct Walk {
     int tx, ty, c0, rp;
     int64_t first, r_end, row0;        // row0: the sample's first row
-    bool mine;                         // the lane has channels
+    int n;                             // channels of the lane: V, fewer at the row's (the slab's) end, 0 if it has none
 };
+
+template <bool ANY, typename R, typename T>
+__device__ __forceinline__ void load_lane(R& raw, const T* p, int n, int c) {
+    if constexpr (ANY) raw.load_some(p, n, c >= 16 / (int)sizeof(T));
+    else raw.load(p);
+}
+template <bool ANY, bool STREAM, int DT, int V>
+__device__ __forceinline__ void store_lane(typename Elem<DT>::T* p, const float (&v)[V], int n) {
+    Raw<DT> raw;
+    raw.set(v);
+    if constexpr (ANY) raw.store_some(p, n);
+    else raw.template store<STREAM>(p);
+}
+// n of a lane whose channels start `left` in front of the end
+template <int V>
+__device__ __forceinline__ int lane_channels(bool on, int left) { return !on || left <= 0 ? 0 : left < V ? left : V; }
 
 // sum over ty of the threads' values (red[ty * width + tx], every thread's written): at red[tx] behind it, in a fixed order
 template <typename P>
@@ -119,7 +141,7 @@ __device__ __forceinline__ void fold_rows(P* red, int tx, int ty, int width, int
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 
 // a thread's moments over its rows, and (KEEP) the checkpoint of them; every thread of the work-group makes the same trips
-template <int DT, int V, bool KEEP>
+template <int DT, bool ANY, bool KEEP, int V>
 __device__ __forceinline__ void walk_sums(const typename Elem<DT>::T* __restrict__ x, int8_t* __restrict__ codes,
                                           uint8_t* __restrict__ scales, const Walk& w, const GnShape& p, double (&sx)[V], double (&sxx)[V]) {
     constexpr int LB = kBlk8 / V;
@@ -127,9 +149,9 @@ __device__ __forceinline__ void walk_sums(const typename Elem<DT>::T* __restrict
 #pragma unroll
     for (int j = 0; j < V; ++j) k[j] = s1[j] = s2[j] = 0.0f;
     const int64_t begin = w.first + kQ * w.ty;
-    if (w.mine && begin < w.r_end) {
-        Raw<DT, V> raw;
-        raw.load(x + (w.row0 + begin) * p.c + w.c0);
+    if (w.n > 0 && begin < w.r_end) {
+        Raw<DT> raw;
+        load_lane<ANY>(raw, x + (w.row0 + begin) * p.c + w.c0, w.n, p.c);
         raw.get(k);
     }
     int64_t count = 0;
@@ -137,12 +159,12 @@ __device__ __forceinline__ void walk_sums(const typename Elem<DT>::T* __restrict
     const bool kept = KEEP && w.ty < w.rp && cb < p.blocks;
     for (int64_t r0 = w.first; r0 < w.r_end; r0 += kQ * w.rp) {
         const int64_t r = r0 + kQ * w.ty;
-        Raw<DT, V> raw[kQ];
-        const int have = !w.mine || r >= w.r_end ? 0 : w.r_end - r < kQ ? (int)(w.r_end - r) : kQ;
+        Raw<DT> raw[kQ];
+        const int have = w.n <= 0 || r >= w.r_end ? 0 : w.r_end - r < kQ ? (int)(w.r_end - r) : kQ;
 #pragma unroll
         for (int i = 0; i < kQ; ++i) {
             raw[i].zero();
-            if (i < have) raw[i].load(x + (w.row0 + r + i) * p.c + w.c0);
+            if (i < have) load_lane<ANY>(raw[i], x + (w.row0 + r + i) * p.c + w.c0, w.n, p.c);
         }
         unsigned e[kQ];
         if constexpr (KEEP)
@@ -164,17 +186,9 @@ __device__ __forceinline__ void walk_sums(const typename Elem<DT>::T* __restrict
                 if (kept && r + i < w.r_end) store_codes<V>(codes + (w.row0 + r + i) * p.blocks * kBlk8 + w.c0, v, block8_inverse(e[i]));
         }
         if constexpr (KEEP)
-            if (kept && w.c0 % kBlk8 == 0) {
-                uint8_t* to = scales + (int64_t)cb * p.rows + w.row0 + r;
-                if (r + kQ <= w.r_end) {
-                    const unsigned word = e[0] | (e[1] << 8) | (e[2] << 16) | (e[3] << 24);
-                    __builtin_memcpy(to, &word, 4);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kQ; ++i)
-                        if (r + i < w.r_end) to[i] = (uint8_t)e[i];
-                }
-            }
+            if (kept && w.c0 % kBlk8 == 0 && r < w.r_end)
+                store_exponents(scales + (int64_t)cb * p.rows + w.row0 + r, e[0] | (e[1] << 8) | (e[2] << 16) | (e[3] << 24),
+                                w.r_end - r < kQ ? (int)(w.r_end - r) : kQ);
     }
     const double m = (double)count;
 #pragma unroll
@@ -193,17 +207,17 @@ __device__ __forceinline__ float2 moments(double a, double b, double m, float ep
     return float2{(float)mu, (float)(1.0 / sqrt(var + (double)eps))};
 }
 
-template <int DT, int V, int ACT, bool STREAM>
+template <int DT, bool ANY, int ACT, bool STREAM, int V>
 __device__ __forceinline__ void walk_apply(const typename Elem<DT>::T* __restrict__ x, typename Elem<DT>::T* __restrict__ y, const Walk& w,
                                            const GnShape& p, const float (&mu)[V], const float (&a)[V], const float (&b)[V], float slope,
                                            float scale) {
     for (int64_t r = w.first + kQ * w.ty; r < w.r_end; r += kQ * w.rp) {
         const int64_t at = (w.row0 + r) * p.c + w.c0;
         const int have = w.r_end - r < kQ ? (int)(w.r_end - r) : kQ;
-        Raw<DT, V> raw[kQ];
+        Raw<DT> raw[kQ];
 #pragma unroll
         for (int i = 0; i < kQ; ++i)
-            if (i < have) raw[i].load(x + at + (int64_t)i * p.c);
+            if (i < have) load_lane<ANY>(raw[i], x + at + (int64_t)i * p.c, w.n, p.c);
 #pragma unroll
         for (int i = 0; i < kQ; ++i)
             if (i < have) {
@@ -211,15 +225,16 @@ __device__ __forceinline__ void walk_apply(const typename Elem<DT>::T* __restric
                 raw[i].get(v);
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[j] = Act<ACT>::value(fmaf(v[j] - mu[j], a[j], b[j]), slope, scale);
-                store_vec<DT, V, STREAM>(y + at + (int64_t)i * p.c, v);
+                store_lane<ANY, STREAM, DT>(y + at + (int64_t)i * p.c, v, w.n);
             }
     }
 }
 
 // record [n][chunk][unit]: sum x and sum x^2 of the unit over the chunk's rows
-template <int DT, int V, bool KEEP>
+template <int DT, bool ANY, bool KEEP>
 __global__ __launch_bounds__(kBlock) void gn_sums_kernel(const typename Elem<DT>::T* __restrict__ x, double2* __restrict__ rec,
                                                          int8_t* __restrict__ codes, uint8_t* __restrict__ scales, const GnShape p) {
+    constexpr int V = Elem<DT>::kVec;
     __shared__ double2 red[kBlock];
     const int n = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
     Walk w;
@@ -232,9 +247,9 @@ __global__ __launch_bounds__(kBlock) void gn_sums_kernel(const typename Elem<DT>
     const bool whole = p.cg % V == 0;
     for (int lane0 = 0; lane0 < p.lanes; lane0 += p.tile) {
         w.c0 = (lane0 + w.tx) * V;
-        w.mine = w.ty < w.rp && w.c0 < p.c;
+        w.n = lane_channels<V>(w.ty < w.rp, p.c - w.c0);
         double sx[V], sxx[V];
-        walk_sums<DT, V, KEEP>(x, codes, scales, w, p, sx, sxx);
+        walk_sums<DT, ANY, KEEP>(x, codes, scales, w, p, sx, sxx);
         const int rounds = whole ? 1 : V;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -247,7 +262,7 @@ __global__ __launch_bounds__(kBlock) void gn_sums_kernel(const typename Elem<DT>
             red[tid] = t;
             fold_rows(red, w.tx, w.ty, p.tile, p.rp, w.ty < p.rp);
             const int unit = whole ? lane0 + w.tx : w.c0 + j;
-            if (w.ty == 0 && w.c0 < p.c) rec[((int64_t)n * p.chunks + chunk) * p.units + unit] = red[w.tx];
+            if (w.ty == 0 && j < w.n) rec[((int64_t)n * p.chunks + chunk) * p.units + unit] = red[w.tx];
         }
     }
 }
@@ -281,12 +296,13 @@ __global__ __launch_bounds__(kWave) void gn_totals_kernel(const double2* __restr
 
 // TOTALS: the statistics too, from the sample's records -- each work-group for itself, where they are few
 constexpr int kFoldGroups = 256, kFoldRecords = 1024;
-template <int DT, int V, int ACT, bool TOTALS>
+template <int DT, bool ANY, int ACT, bool TOTALS>
 __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const typename Elem<DT>::T* __restrict__ x, const double2* __restrict__ rec,
                                                           float* __restrict__ mean, float* __restrict__ rstd,
                                                           const float* __restrict__ weight, const float* __restrict__ bias,
                                                           typename Elem<DT>::T* __restrict__ y, float eps, float slope, float scale,
                                                           const GnShape p) {
+    constexpr int V = Elem<DT>::kVec;
     const int n = (int)gridDim.y - 1 - (int)blockIdx.y, chunk = (int)gridDim.x - 1 - (int)blockIdx.x, tid = threadIdx.x;
     Walk w;
     w.tx = tid % p.tile;
@@ -330,12 +346,13 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const typename Elem<DT
     if (w.ty >= w.rp) return;
     for (int lane0 = 0; lane0 < p.lanes; lane0 += p.tile) {
         w.c0 = (lane0 + w.tx) * V;
-        if (w.c0 >= p.c) return;
+        w.n = lane_channels<V>(true, p.c - w.c0);
+        if (w.n == 0) return;
         float mu[V], a[V], b[V];
         int g[V];
-        groups_of<V>(w.c0, p.cg, g);
-        load_param<V>(weight, w.c0, 1.0f, a);
-        load_param<V>(bias, w.c0, 0.0f, b);
+        groups_of<V>(w.c0, p.cg, p.groups, g);
+        load_param<V>(weight, w.c0, w.n, 1.0f, a);
+        load_param<V>(bias, w.c0, w.n, 0.0f, b);
         float2 s;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -347,7 +364,7 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const typename Elem<DT
             a[j] *= s.y * Act<ACT>::kArg;
             b[j] *= Act<ACT>::kArg;
         }
-        walk_apply<DT, V, ACT, true>(x, y, w, p, mu, a, b, slope, scale);
+        walk_apply<DT, ANY, ACT, true>(x, y, w, p, mu, a, b, slope, scale);
     }
 }
 
@@ -365,16 +382,17 @@ __device__ __forceinline__ Walk slab_walk(const GnShape& p, int& g0, int& gs, in
     w.first = 0;
     w.r_end = p.l;
     w.c0 = g0 * p.cg + w.tx * V;
-    w.mine = w.ty < w.rp && w.tx * V < width;
+    w.n = lane_channels<V>(w.ty < w.rp, width - w.tx * V);
     return w;
 }
 
-template <int DT, int V, int ACT, bool KEEP>
+template <int DT, bool ANY, int ACT, bool KEEP>
 __global__ __launch_bounds__(kFused) void gn_fused_kernel(const typename Elem<DT>::T* __restrict__ x, const float* __restrict__ weight,
                                                           const float* __restrict__ bias, typename Elem<DT>::T* __restrict__ y,
                                                           float* __restrict__ mean, float* __restrict__ rstd, int8_t* __restrict__ codes,
                                                           uint8_t* __restrict__ scales, float eps, float slope, float scale,
                                                           const GnShape p) {
+    constexpr int V = Elem<DT>::kVec;
     __shared__ double2 red[kFused];
     __shared__ double2 unit[kFused];
     __shared__ float2 stat[kFused];
@@ -383,7 +401,7 @@ __global__ __launch_bounds__(kFused) void gn_fused_kernel(const typename Elem<DT
     const int tid = threadIdx.x;
     const bool whole = p.cg % V == 0;
     double sx[V], sxx[V];
-    walk_sums<DT, V, KEEP>(x, codes, scales, w, p, sx, sxx);
+    walk_sums<DT, ANY, KEEP>(x, codes, scales, w, p, sx, sxx);
     // unit sums of the slab: of its channel vectors, or of its channels (at most kFused of them: gn_slab)
     const int rounds = whole ? 1 : V;
 #pragma unroll
@@ -396,7 +414,7 @@ __global__ __launch_bounds__(kFused) void gn_fused_kernel(const typename Elem<DT
         __syncthreads();
         red[tid] = t;
         fold_rows(red, w.tx, w.ty, p.tile, p.rp, w.ty < p.rp);
-        if (w.ty == 0 && w.mine) unit[whole ? w.tx : w.tx * V + j] = red[w.tx];
+        if (w.ty == 0 && j < w.n) unit[whole ? w.tx : w.tx * V + j] = red[w.tx];
     }
     __syncthreads();
     const int per = whole ? p.cg / V : p.cg;
@@ -412,45 +430,42 @@ __global__ __launch_bounds__(kFused) void gn_fused_kernel(const typename Elem<DT
         rstd[(int64_t)blockIdx.y * p.groups + g0 + g] = s.y;
     }
     __syncthreads();
-    if (!w.mine) return;
+    if (w.n == 0) return;
     float mu[V], a[V], b[V];
+    int g[V];
+    groups_of<V>(w.tx * V, p.cg, gs, g);
+    load_param<V>(weight, w.c0, w.n, 1.0f, a);
+    load_param<V>(bias, w.c0, w.n, 0.0f, b);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float2 s = stat[(w.tx * V + j) / p.cg];
+        const float2 s = stat[g[j]];
         mu[j] = s.x;
-        a[j] = s.y * (weight ? weight[w.c0 + j] : 1.0f) * Act<ACT>::kArg;
-        b[j] = (bias ? bias[w.c0 + j] : 0.0f) * Act<ACT>::kArg;
+        a[j] *= s.y * Act<ACT>::kArg;
+        b[j] *= Act<ACT>::kArg;
     }
-    walk_apply<DT, V, ACT, false>(x, y, w, p, mu, a, b, slope, scale);
+    walk_apply<DT, ANY, ACT, false>(x, y, w, p, mu, a, b, slope, scale);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------------
 
 // kQ rows of the input: from the tensor, or (KEPT) from their codes
-template <int DT, int V, bool KEPT>
+template <int DT, bool ANY, bool KEPT>
 struct Input {
-    Raw<DT, V> raw[kQ];
+    static constexpr int V = Elem<DT>::kVec;
+    Raw<DT> raw[kQ];
     RawCodes<V> code[kQ];
     unsigned e;
     __device__ __forceinline__ void load(const typename Elem<DT>::T* x, const int8_t* codes, const uint8_t* scales, int64_t row, int c0,
-                                         int have, const GnShape& p) {
+                                         int n, int have, const GnShape& p) {
         if constexpr (KEPT) {
 #pragma unroll
             for (int i = 0; i < kQ; ++i)
                 if (i < have) code[i].load(codes + (row + i) * p.blocks * kBlk8 + c0);
-            const uint8_t* from = scales + (int64_t)(c0 / kBlk8) * p.rows + row;
-            e = 0;
-            if (have == kQ) {
-                __builtin_memcpy(&e, from, 4);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kQ; ++i)
-                    if (i < have) e |= (unsigned)from[i] << (8 * i);
-            }
+            e = load_exponents(scales + (int64_t)(c0 / kBlk8) * p.rows + row, have);
         } else {
 #pragma unroll
             for (int i = 0; i < kQ; ++i)
-                if (i < have) raw[i].load(x + (row + i) * p.c + c0);
+                if (i < have) load_lane<ANY>(raw[i], x + (row + i) * p.c + c0, n, p.c);
         }
     }
     __device__ __forceinline__ void get(int i, float (&v)[V]) const {
@@ -466,19 +481,19 @@ struct Affine {
 };
 
 // a thread's sums over its rows of g = gy act'(z) and of g (x - mean)
-template <int DT, int V, int ACT, bool KEPT>
+template <int DT, bool ANY, int ACT, bool KEPT, int V>
 __device__ __forceinline__ void walk_bwd_sums(const typename Elem<DT>::T* __restrict__ gy, const typename Elem<DT>::T* __restrict__ x,
                                               const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const Walk& w,
                                               const GnShape& p, const Affine<V>& f, float slope, float (&s1)[V], float (&s2)[V]) {
     for (int64_t r = w.first + kQ * w.ty; r < w.r_end; r += kQ * w.rp) {
         const int64_t row = w.row0 + r;
         const int have = w.r_end - r < kQ ? (int)(w.r_end - r) : kQ;
-        Input<DT, V, KEPT> in;
-        Raw<DT, V> raw[kQ];
-        in.load(x, codes, scales, row, w.c0, have, p);
+        Input<DT, ANY, KEPT> in;
+        Raw<DT> raw[kQ];
+        in.load(x, codes, scales, row, w.c0, w.n, have, p);
 #pragma unroll
         for (int i = 0; i < kQ; ++i)
-            if (i < have) raw[i].load(gy + (row + i) * p.c + w.c0);
+            if (i < have) load_lane<ANY>(raw[i], gy + (row + i) * p.c + w.c0, w.n, p.c);
 #pragma unroll
         for (int i = 0; i < kQ; ++i)
             if (i < have) {
@@ -497,7 +512,7 @@ __device__ __forceinline__ void walk_bwd_sums(const typename Elem<DT>::T* __rest
 }
 
 // gx = ga * g + (x - mean) * gd + ge, g as above
-template <int DT, int V, int ACT, bool KEPT, bool STREAM>
+template <int DT, bool ANY, int ACT, bool KEPT, bool STREAM, int V>
 __device__ __forceinline__ void walk_bwd_apply(const typename Elem<DT>::T* __restrict__ gy, const typename Elem<DT>::T* __restrict__ x,
                                                const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                typename Elem<DT>::T* __restrict__ gx, const Walk& w, const GnShape& p, const Affine<V>& f,
@@ -505,12 +520,12 @@ __device__ __forceinline__ void walk_bwd_apply(const typename Elem<DT>::T* __res
     for (int64_t r = w.first + kQ * w.ty; r < w.r_end; r += kQ * w.rp) {
         const int64_t row = w.row0 + r;
         const int have = w.r_end - r < kQ ? (int)(w.r_end - r) : kQ;
-        Input<DT, V, KEPT> in;
-        Raw<DT, V> raw[kQ];
-        in.load(x, codes, scales, row, w.c0, have, p);
+        Input<DT, ANY, KEPT> in;
+        Raw<DT> raw[kQ];
+        in.load(x, codes, scales, row, w.c0, w.n, have, p);
 #pragma unroll
         for (int i = 0; i < kQ; ++i)
-            if (i < have) raw[i].load(gy + (row + i) * p.c + w.c0);
+            if (i < have) load_lane<ANY>(raw[i], gy + (row + i) * p.c + w.c0, w.n, p.c);
 #pragma unroll
         for (int i = 0; i < kQ; ++i)
             if (i < have) {
@@ -523,7 +538,7 @@ __device__ __forceinline__ void walk_bwd_apply(const typename Elem<DT>::T* __res
                     const float dz = g[j] * Act<ACT>::derivative(fmaf(d, f.a[j], f.b[j]), slope);
                     v[j] = fmaf(ga[j], dz, fmaf(d, gd[j], ge[j]));
                 }
-                store_vec<DT, V, STREAM>(gx + (row + i) * p.c + w.c0, v);
+                store_lane<ANY, STREAM, DT>(gx + (row + i) * p.c + w.c0, v, w.n);
             }
     }
 }
@@ -534,11 +549,11 @@ struct BwdIn {
 };
 
 template <int V, int ACT>
-__device__ __forceinline__ void load_affine(const BwdIn& in, int64_t n, int c0, const GnShape& p, Affine<V>& f) {
+__device__ __forceinline__ void load_affine(const BwdIn& in, int64_t n, int c0, int channels, const GnShape& p, Affine<V>& f) {
     int g[V];
-    groups_of<V>(c0, p.cg, g);
-    load_param<V>(in.weight, c0, 1.0f, f.a);
-    load_param<V>(in.bias, c0, 0.0f, f.b);
+    groups_of<V>(c0, p.cg, p.groups, g);
+    load_param<V>(in.weight, c0, channels, 1.0f, f.a);
+    load_param<V>(in.bias, c0, channels, 0.0f, f.b);
     float mu = 0.0f, rs = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -553,11 +568,12 @@ __device__ __forceinline__ void load_affine(const BwdIn& in, int64_t n, int c0, 
 }
 
 // record [n][chunk][channel]: the two sums over the chunk's rows
-template <int DT, int V, int ACT, bool KEPT>
+template <int DT, bool ANY, int ACT, bool KEPT>
 __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const typename Elem<DT>::T* __restrict__ gy,
                                                              const typename Elem<DT>::T* __restrict__ x,
                                                              const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                              const BwdIn in, float2* __restrict__ rec, float slope, const GnShape p) {
+    constexpr int V = Elem<DT>::kVec;
     __shared__ float2 red[V][kBlock];
     const int n = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
     Walk w;
@@ -569,14 +585,14 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const typename Elem
     w.r_end = w.first + p.chunk_rows < p.l ? w.first + p.chunk_rows : p.l;
     for (int lane0 = 0; lane0 < p.lanes; lane0 += p.tile) {
         w.c0 = (lane0 + w.tx) * V;
-        w.mine = w.ty < w.rp && w.c0 < p.c;
+        w.n = lane_channels<V>(w.ty < w.rp, p.c - w.c0);
         float s1[V], s2[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
-        if (w.mine) {
+        if (w.n > 0) {
             Affine<V> f;
-            load_affine<V, ACT>(in, n, w.c0, p, f);
-            walk_bwd_sums<DT, V, ACT, KEPT>(gy, x, codes, scales, w, p, f, slope, s1, s2);
+            load_affine<V, ACT>(in, n, w.c0, w.n, p, f);
+            walk_bwd_sums<DT, ANY, ACT, KEPT>(gy, x, codes, scales, w, p, f, slope, s1, s2);
         }
         __syncthreads();
 #pragma unroll
@@ -593,9 +609,10 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(const typename Elem
                     red[j][tid].y += o.y;
                 }
         }
-        if (w.ty == 0 && w.mine)
+        if (w.ty == 0)
 #pragma unroll
-            for (int j = 0; j < V; ++j) rec[((int64_t)n * p.chunks + chunk) * p.c + w.c0 + j] = red[j][tid];
+            for (int j = 0; j < V; ++j)
+                if (j < w.n) rec[((int64_t)n * p.chunks + chunk) * p.c + w.c0 + j] = red[j][tid];
     }
 }
 
@@ -665,7 +682,7 @@ __device__ __forceinline__ void bwd_factors(float rs, float2 m, float w, float s
     ge = -rs * m.x;
 }
 
-template <int DT, int V, int ACT, bool KEPT>
+template <int DT, bool ANY, int ACT, bool KEPT>
 __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const typename Elem<DT>::T* __restrict__ gy,
                                                               const typename Elem<DT>::T* __restrict__ x,
                                                               const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
@@ -673,6 +690,7 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const typename Ele
                                                               const float2* __restrict__ totals, float* __restrict__ gw,
                                                               float* __restrict__ gb, typename Elem<DT>::T* __restrict__ gx, float slope,
                                                               float scale, const GnShape p) {
+    constexpr int V = Elem<DT>::kVec;
     const int n = (int)gridDim.y - 1 - (int)blockIdx.y, chunk = (int)gridDim.x - 1 - (int)blockIdx.x, tid = threadIdx.x;
     if (totals) {                                                  // gw and gb on the way, 256 channels a work-group
         const int blocks = (int)(gridDim.x * gridDim.y);
@@ -689,13 +707,14 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const typename Ele
     if (w.ty >= w.rp) return;
     for (int lane0 = 0; lane0 < p.lanes; lane0 += p.tile) {
         w.c0 = (lane0 + w.tx) * V;
-        if (w.c0 >= p.c) return;
+        w.n = lane_channels<V>(true, p.c - w.c0);
+        if (w.n == 0) return;
         Affine<V> f;
-        load_affine<V, ACT>(in, n, w.c0, p, f);
+        load_affine<V, ACT>(in, n, w.c0, w.n, p, f);
         float ga[V], gd[V], ge[V];
         int g[V];
-        groups_of<V>(w.c0, p.cg, g);
-        load_param<V>(in.weight, w.c0, 1.0f, ga);
+        groups_of<V>(w.c0, p.cg, p.groups, g);
+        load_param<V>(in.weight, w.c0, w.n, 1.0f, ga);
         float rs = 0.0f;
         float2 m{0.0f, 0.0f};
 #pragma unroll
@@ -706,18 +725,19 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const typename Ele
             }
             bwd_factors<V>(rs, m, ga[j], scale, ga[j], gd[j], ge[j]);
         }
-        walk_bwd_apply<DT, V, ACT, KEPT, true>(gy, x, codes, scales, gx, w, p, f, ga, gd, ge, slope);
+        walk_bwd_apply<DT, ANY, ACT, KEPT, true>(gy, x, codes, scales, gx, w, p, f, ga, gd, ge, slope);
     }
 }
 
 // one launch: a sample's slab of groups; totals [n][c] for the weights' kernel, or (one sample) gw and gb themselves
-template <int DT, int V, int ACT, bool KEPT>
+template <int DT, bool ANY, int ACT, bool KEPT>
 __global__ __launch_bounds__(kFused) void gn_bwd_fused_kernel(const typename Elem<DT>::T* __restrict__ gy,
                                                               const typename Elem<DT>::T* __restrict__ x,
                                                               const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                               const BwdIn in, float2* __restrict__ totals, float* __restrict__ gw,
                                                               float* __restrict__ gb, typename Elem<DT>::T* __restrict__ gx, float slope,
                                                               float scale, const GnShape p) {
+    constexpr int V = Elem<DT>::kVec;
     __shared__ float2 red[V][kFused];
     __shared__ float2 mean[kFused];
     int g0, gs, width;
@@ -727,9 +747,9 @@ __global__ __launch_bounds__(kFused) void gn_bwd_fused_kernel(const typename Ele
     float s1[V], s2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
-    if (w.mine) {
-        load_affine<V, ACT>(in, blockIdx.y, w.c0, p, f);
-        walk_bwd_sums<DT, V, ACT, KEPT>(gy, x, codes, scales, w, p, f, slope, s1, s2);
+    if (w.n > 0) {
+        load_affine<V, ACT>(in, blockIdx.y, w.c0, w.n, p, f);
+        walk_bwd_sums<DT, ANY, ACT, KEPT>(gy, x, codes, scales, w, p, f, slope, s1, s2);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) red[j][tid] = float2{s1[j], s2[j]};
@@ -764,15 +784,15 @@ __global__ __launch_bounds__(kFused) void gn_bwd_fused_kernel(const typename Ele
         mean[i] = float2{(float)(m1 / m), (float)(m2 / m)};
     }
     __syncthreads();
-    if (!w.mine || !gx) return;
+    if (w.n == 0 || !gx) return;
     float ga[V], gd[V], ge[V];
+    int g[V];
+    groups_of<V>(w.tx * V, p.cg, gs, g);
+    load_param<V>(in.weight, w.c0, w.n, 1.0f, ga);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int g = (w.tx * V + j) / p.cg;
-        bwd_factors<V>(in.rstd[(int64_t)blockIdx.y * p.groups + g0 + g], mean[g], in.weight ? in.weight[w.c0 + j] : 1.0f, scale, ga[j],
-                       gd[j], ge[j]);
-    }
-    walk_bwd_apply<DT, V, ACT, KEPT, false>(gy, x, codes, scales, gx, w, p, f, ga, gd, ge, slope);
+    for (int j = 0; j < V; ++j)
+        bwd_factors<V>(in.rstd[(int64_t)blockIdx.y * p.groups + g0 + g[j]], mean[g[j]], ga[j], scale, ga[j], gd[j], ge[j]);
+    walk_bwd_apply<DT, ANY, ACT, KEPT, false>(gy, x, codes, scales, gx, w, p, f, ga, gd, ge, slope);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
@@ -784,19 +804,21 @@ bool gn_shape_ok(int64_t n, int64_t l, int64_t c, int64_t groups) {
            c % groups == 0 && l <= ((int64_t)1 << 40) / c;
 }
 
-// Groups of a one-launch work-group: whole vectors, whole 8-bit blocks where it writes them (or the whole row), at least 64 bytes of a
-// row (one group's share is often less, and every 64-byte piece is read whole); 0 if there is no such slab.
-int gn_slab(int64_t c, int64_t groups, int v, int esize, bool keep) {
-    const int64_t cg = c / groups;
+// Groups of a one-launch work-group: at least 64 bytes of a row (one group's share is often less, and every 64-byte piece is read
+// whole); with codes whole 8-bit blocks where it writes them and whole vectors where it reads them; 0 if there is no such slab.
+enum GnCodes { kNoCodes, kWriteCodes, kReadCodes };
+int gn_slab(int64_t c, int64_t groups, int v, int esize, GnCodes codes) {
+    const int64_t cg = c / groups, whole = codes == kWriteCodes ? kBlk8 : codes == kReadCodes ? v : 1;
     for (int64_t s = 1; s <= groups; ++s) {
         const int64_t w = s * cg;
         if (w > kFused || s > kFused) return 0;                    // a lane, a unit and a group at most for each thread
-        if (s == groups || (w % v == 0 && (!keep || w % kBlk8 == 0) && w * esize >= 64)) return (int)s;
+        if (s == groups || (w % whole == 0 && w * esize >= 64)) return (int)s;
     }
     return 0;
 }
 
-GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int v, int esize, bool keep) {
+GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int esize, GnCodes codes) {
+    const int v = 16 / esize;
     GnShape p;
     p.l = l;
     p.rows = n * l;
@@ -805,7 +827,7 @@ GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int v, int esiz
     p.cg = (int)(c / groups);
     p.blocks = (int)ceil_div64(c, kBlk8);
     p.units = p.cg % v == 0 ? (int)c / v : (int)c;
-    p.slab = gn_slab(c, groups, v, esize, keep);
+    p.slab = gn_slab(c, groups, v, esize, codes);
     p.slabs = p.slab ? (int)ceil_div64(groups, p.slab) : 0;
     // One launch where a thread of kFused makes at most 8 / kQ trips over its slab, twice; 16 where the whole tensor is so small (4 MB)
     // that launches are what costs.  (knob 0, for tests: never)
@@ -813,8 +835,11 @@ GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int v, int esiz
         const int64_t trips = ceil_div64(l * p.slab * p.cg, (int64_t)kFused * v) * tuning_knob("SAE_GN_ONE_LAUNCH", 1);
         if (trips == 0 || trips > (n * l * c * esize <= ((int64_t)4 << 20) ? 16 : 8)) p.slab = 0;
     }
+    // lanes of so many channels; a walk that writes codes has all lanes of a block
+    auto lanes_of = [&](int64_t w) { return (int)(codes == kWriteCodes ? ceil_div64(w, kBlk8) * (kBlk8 / v) : ceil_div64(w, v)); };
+    p.any = c % v != 0 || (p.slab && (int64_t)p.slab * p.cg % v != 0);
     if (p.slab) {
-        p.lanes = (int)ceil_div64((int64_t)p.slab * p.cg, kBlk8) * (kBlk8 / v);
+        p.lanes = lanes_of((int64_t)p.slab * p.cg);
         p.tile = p.lanes;
         p.rp = kFused / p.tile;
         while (p.rp > 1 && (int64_t)(p.rp / 2) * kQ >= l) p.rp /= 2;          // (no more threads than rows)
@@ -822,7 +847,7 @@ GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int v, int esiz
         p.chunks = 1;
         return p;
     }
-    p.lanes = p.blocks * (kBlk8 / v);
+    p.lanes = lanes_of(c);
     p.tile = p.lanes < kBlock ? p.lanes : kBlock;
     p.rp = kBlock / p.tile;
     // Up to 8 work-groups per CU over the whole batch, while each thread has four trips of kQ rows (one trip alone is all prologue:
@@ -858,37 +883,37 @@ struct GnArgs {
     hipStream_t stream;
 };
 
-template <int DT, int V, int ACT>
+template <int DT, bool ANY, int ACT>
 void gn_forward_as(const GnArgs& a, const GnShape& p) {
     using T = typename Elem<DT>::T;
     if (p.slab) {
         const dim3 grid((unsigned)p.slabs, (unsigned)a.n), block((unsigned)(p.tile * p.rp));
         if (a.codes)
-            hipLaunchKernelGGL((gn_fused_kernel<DT, V, ACT, true>), grid, block, 0, a.stream, (const T*)a.x, a.weight, a.bias, (T*)a.out,
+            hipLaunchKernelGGL((gn_fused_kernel<DT, ANY, ACT, true>), grid, block, 0, a.stream, (const T*)a.x, a.weight, a.bias, (T*)a.out,
                                a.mean, a.rstd, a.codes, a.scales, a.eps, a.slope, a.scale, p);
         else
-            hipLaunchKernelGGL((gn_fused_kernel<DT, V, ACT, false>), grid, block, 0, a.stream, (const T*)a.x, a.weight, a.bias,
+            hipLaunchKernelGGL((gn_fused_kernel<DT, ANY, ACT, false>), grid, block, 0, a.stream, (const T*)a.x, a.weight, a.bias,
                                (T*)a.out, a.mean, a.rstd, a.codes, a.scales, a.eps, a.slope, a.scale, p);
         return;
     }
     const dim3 grid((unsigned)p.chunks, (unsigned)a.n), block(kBlock);
     double2* rec = (double2*)a.ws;
     if (a.codes)
-        hipLaunchKernelGGL((gn_sums_kernel<DT, V, true>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
+        hipLaunchKernelGGL((gn_sums_kernel<DT, ANY, true>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
     else
-        hipLaunchKernelGGL((gn_sums_kernel<DT, V, false>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
+        hipLaunchKernelGGL((gn_sums_kernel<DT, ANY, false>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
     if (p.groups <= kFoldGroups && p.chunks * p.units <= kFoldRecords) {
-        hipLaunchKernelGGL((gn_apply_kernel<DT, V, ACT, true>), grid, block, 0, a.stream, (const T*)a.x, (const double2*)rec, a.mean,
+        hipLaunchKernelGGL((gn_apply_kernel<DT, ANY, ACT, true>), grid, block, 0, a.stream, (const T*)a.x, (const double2*)rec, a.mean,
                            a.rstd, a.weight, a.bias, (T*)a.out, a.eps, a.slope, a.scale, p);
         return;
     }
     hipLaunchKernelGGL(gn_totals_kernel, dim3((unsigned)p.groups, (unsigned)a.n), dim3(kWave), 0, a.stream, (const double2*)rec,
                        a.mean, a.rstd, a.eps, p);
-    hipLaunchKernelGGL((gn_apply_kernel<DT, V, ACT, false>), grid, block, 0, a.stream, (const T*)a.x, (const double2*)rec, a.mean,
+    hipLaunchKernelGGL((gn_apply_kernel<DT, ANY, ACT, false>), grid, block, 0, a.stream, (const T*)a.x, (const double2*)rec, a.mean,
                        a.rstd, a.weight, a.bias, (T*)a.out, a.eps, a.slope, a.scale, p);
 }
 
-template <int DT, int V, int ACT, bool KEPT>
+template <int DT, bool ANY, int ACT, bool KEPT>
 void gn_backward_as(const GnArgs& a, const GnShape& p) {
     using T = typename Elem<DT>::T;
     const BwdIn in{a.mean, a.rstd, a.weight, a.bias};
@@ -896,7 +921,7 @@ void gn_backward_as(const GnArgs& a, const GnShape& p) {
     if (p.slab) {
         const dim3 grid((unsigned)p.slabs, (unsigned)a.n), block((unsigned)(p.tile * p.rp));
         float2* totals = a.n > 1 && weights ? (float2*)a.ws : nullptr;
-        hipLaunchKernelGGL((gn_bwd_fused_kernel<DT, V, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
+        hipLaunchKernelGGL((gn_bwd_fused_kernel<DT, ANY, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
                            (const int8_t*)a.codes, (const uint8_t*)a.scales, in, totals, totals ? nullptr : a.gw,
                            totals ? nullptr : a.gb, (T*)a.out, a.slope, a.scale, p);
         if (totals)
@@ -908,12 +933,12 @@ void gn_backward_as(const GnArgs& a, const GnShape& p) {
     float2* rec = (float2*)a.ws;
     float2* totals = rec + a.n * p.chunks * (int64_t)p.c;
     float2* means = totals + a.n * p.c;
-    hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, V, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, ANY, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
                        (const int8_t*)a.codes, (const uint8_t*)a.scales, in, rec, a.slope, p);
     hipLaunchKernelGGL(gn_bwd_totals_kernel, dim3((unsigned)p.groups, (unsigned)a.n), block, 0, a.stream, (const float2*)rec,
                        a.weight, (const float*)a.rstd, totals, means, a.scale, p);
     if (a.out)
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, V, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, ANY, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
                            (const int8_t*)a.codes, (const uint8_t*)a.scales, in, (const float2*)means,
                            weights ? (const float2*)totals : (const float2*)nullptr, a.gw, a.gb, (T*)a.out, a.slope, a.scale, p);
     else
@@ -921,41 +946,38 @@ void gn_backward_as(const GnArgs& a, const GnShape& p) {
                            a.gw, a.gb, (int)a.n, p.c);
 }
 
-// V channels per lane in 16-byte accesses where the rows allow it, one channel where not
-bool gn_vector(int64_t c, int32_t dtype) { return c % (16 / elem_bytes(dtype)) == 0; }
-
-template <int DT, int V, int ACT>
+template <int DT, bool ANY, int ACT>
 void gn_run(const GnArgs& a, const GnShape& p, bool backward) {
-    if (!backward) gn_forward_as<DT, V, ACT>(a, p);
-    else if (a.codes) gn_backward_as<DT, V, ACT, true>(a, p);
-    else gn_backward_as<DT, V, ACT, false>(a, p);
+    if (!backward) gn_forward_as<DT, ANY, ACT>(a, p);
+    else if (a.codes) gn_backward_as<DT, ANY, ACT, true>(a, p);
+    else gn_backward_as<DT, ANY, ACT, false>(a, p);
 }
 
-template <int DT, int V>
+template <int DT, bool ANY>
 void gn_run(const GnArgs& a, const GnShape& p, bool backward) {
-    if (a.act == SAE_ACT_LRELU) gn_run<DT, V, SAE_ACT_LRELU>(a, p, backward);
-    else if (a.act == SAE_ACT_SILU) gn_run<DT, V, SAE_ACT_SILU>(a, p, backward);
-    else gn_run<DT, V, SAE_ACT_NONE>(a, p, backward);
+    if (a.act == SAE_ACT_LRELU) gn_run<DT, ANY, SAE_ACT_LRELU>(a, p, backward);
+    else if (a.act == SAE_ACT_SILU) gn_run<DT, ANY, SAE_ACT_SILU>(a, p, backward);
+    else gn_run<DT, ANY, SAE_ACT_NONE>(a, p, backward);
 }
 
 template <int DT>
-void gn_run(const GnArgs& a, const GnShape& p, bool vec, bool backward) {
-    if (vec) gn_run<DT, Elem<DT>::kVec>(a, p, backward);
-    else gn_run<DT, 1>(a, p, backward);
+void gn_run(const GnArgs& a, const GnShape& p, bool backward) {
+    if (p.any) gn_run<DT, true>(a, p, backward);
+    else gn_run<DT, false>(a, p, backward);
 }
 
 int gn_dispatch(const char* what, GnArgs& a, int64_t l, int64_t c, int64_t groups, int32_t dtype, int64_t ws_bytes, bool backward) {
-    const bool vec = gn_vector(c, dtype);
-    const GnShape p = gn_plan(a.n, l, c, groups, vec ? 16 / elem_bytes(dtype) : 1, elem_bytes(dtype), !backward && a.codes);
+    const GnCodes codes = !a.codes ? kNoCodes : backward ? kReadCodes : kWriteCodes;
+    const GnShape p = gn_plan(a.n, l, c, groups, elem_bytes(dtype), codes);
     const int64_t need = gn_workspace(p, a.n, backward);
     if (need > 0 && (!a.ws || ws_bytes < need))
         return fail(SAE_EWORKSPACE, "%s: workspace %lld < %lld bytes (sae_group_norm_act_workspace)", what, (long long)ws_bytes,
                     (long long)need);
     for (const void* t : {a.gy, a.x, (const void*)a.out, (const void*)a.ws, (const void*)a.codes})
         if (!aligned16(t)) return fail(SAE_EINVAL, "%s: tensors must be 16-byte aligned", what);
-    if (dtype == SAE_F32) gn_run<SAE_F32>(a, p, vec, backward);
-    else if (dtype == SAE_BF16) gn_run<SAE_BF16>(a, p, vec, backward);
-    else gn_run<SAE_F16>(a, p, vec, backward);
+    if (dtype == SAE_F32) gn_run<SAE_F32>(a, p, backward);
+    else if (dtype == SAE_BF16) gn_run<SAE_BF16>(a, p, backward);
+    else gn_run<SAE_F16>(a, p, backward);
     return check_launch(what);
 }
 
@@ -966,9 +988,9 @@ using namespace sae;
 
 extern "C" int64_t sae_group_norm_act_workspace(int64_t n, int64_t l, int64_t c, int64_t groups, int32_t dtype, int32_t backward) {
     if (!gn_shape_ok(n, l, c, groups) || !elem_known(dtype) || n == 0 || l == 0) return 0;
-    // (a forward pass that keeps its input has the wider slabs, and is in one launch only where one that does not is too)
-    return gn_workspace(gn_plan(n, l, c, groups, gn_vector(c, dtype) ? 16 / elem_bytes(dtype) : 1, elem_bytes(dtype), !backward), n,
-                        backward != 0);
+    const int64_t without = gn_workspace(gn_plan(n, l, c, groups, elem_bytes(dtype), kNoCodes), n, backward != 0);
+    const int64_t with = gn_workspace(gn_plan(n, l, c, groups, elem_bytes(dtype), backward ? kReadCodes : kWriteCodes), n, backward != 0);
+    return with > without ? with : without;
 }
 
 extern "C" int sae_group_norm_act(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,

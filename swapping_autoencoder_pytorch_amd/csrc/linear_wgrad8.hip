@@ -385,8 +385,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
                 T* const dst = gw + (int64_t)o * p.c + i;
 #pragma unroll
                 for (int n = 0; n < WN; ++n) {
-                    float one[1] = {alpha * acc[m][n][r]};
-                    if (i + n < p.c) store_vec<DT, 1>(dst + n, one);
+                    if (i + n < p.c) store_one<DT>(dst + n, alpha * acc[m][n][r]);
                 }
             } else if (i < ld) {
                 float* const dst = part + ((int64_t)slice * p.out + o) * ld + i;
@@ -403,11 +402,11 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
             for (int j = 0; j < 4; ++j) fold[ar * BM + 4 * oq + j] = sum[j];
         __syncthreads();
         for (int o = tid; o < BM; o += kBlock) {
-            float t[1] = {fold[o]};
-            for (int rq = 1; rq < AG; ++rq) t[0] += fold[rq * BM + o];
+            float t = fold[o];
+            for (int rq = 1; rq < AG; ++rq) t += fold[rq * BM + o];
             if (o0 + o >= p.out) continue;
-            if constexpr (WHOLE) store_vec<DT, 1>(gb + o0 + o, t);
-            else part_b[(int64_t)slice * p.out + o0 + o] = t[0];
+            if constexpr (WHOLE) store_one<DT>(gb + o0 + o, t);
+            else part_b[(int64_t)slice * p.out + o0 + o] = t;
         }
     }
 }
@@ -440,15 +439,14 @@ __global__ __launch_bounds__(kBlock) void linear_wgrad8_reduce_kernel(const floa
         for (int j = 0; j < 4; ++j) one[j] = alpha * (((v[j] + quarter[0][lane][j]) + quarter[1][lane][j]) + quarter[2][lane][j]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float w[1] = {one[j]};
-            if (i + j < p.c) store_vec<DT, 1>(gw + o * p.c + i + j, w);
+            if (i + j < p.c) store_one<DT>(gw + o * p.c + i + j, one[j]);
         }
     }
     const int64_t u = (int64_t)blockIdx.x * kBlock + threadIdx.x;
     if (gb && u < p.out) {
-        float w[1] = {part_b[u]};
-        for (int s = 1; s < p.slices; ++s) w[0] += part_b[(int64_t)s * p.out + u];
-        store_vec<DT, 1>(gb + u, w);
+        float w = part_b[u];
+        for (int s = 1; s < p.slices; ++s) w += part_b[(int64_t)s * p.out + u];
+        store_one<DT>(gb + u, w);
     }
 }
 

@@ -10,7 +10,6 @@ util/util.py:432-436, which raises on ROCm; that gate is not consulted here.)
 same signatures of the CPU oracle (``oracle_*``) and of the emulator build of the kernels
 (tests/emu) for checking; the product never does.
 """
-import contextlib
 import ctypes as C
 import os
 
@@ -202,30 +201,25 @@ class SaeLibrary:
                     "tensor on %s: the MI355X hot path has no CPU implementation (move the model "
                     "and data to a GPU)" % t.device)
 
-    def check_channels_last(self, *tensors):
-        """Tensors of the channels-last operators: f32, bf16 or f16, one type and one device for all, contiguous, 16-byte aligned
-        (`dense` makes them so) and (product) on a GPU."""
-        first = None
-        for t in tensors:
-            if t is None:
-                continue
-            if t.dtype not in element_types():
-                raise SaeError("channels-last kernels take float32, bfloat16 and float16, got %s" % t.dtype)
-            if first is not None and (t.dtype != first.dtype or t.device != first.device):
-                raise SaeError("tensors of one call must share type and device, got %s on %s and %s on %s"
-                               % (first.dtype, first.device, t.dtype, t.device))
-            if not t.is_contiguous() or t.data_ptr() % 16:
-                raise SaeError("internal error: non-contiguous or misaligned tensor reached the C-ABI")
-            if self.device_only and not t.is_cuda:
-                raise SaeError("tensor on %s: the MI355X operators have no CPU implementation" % t.device)
-            first = t if first is None else first
+    def check_channels_last(self, t):
+        """A tensor of the channels-last operators: f32, bf16 or f16, contiguous, 16-byte aligned (`dense` makes it so) and
+        (product) on a GPU.  Returns its type's code."""
+        code = element_types().get(t.dtype)
+        if code is None:
+            raise SaeError("channels-last kernels take float32, bfloat16 and float16, got %s" % t.dtype)
+        if self.device_only and not t.is_cuda:
+            raise SaeError("tensor on %s: the MI355X operators have no CPU implementation" % t.device)
+        return code
 
-    def device_of(self, t):
-        """Context in which launches go to the tensor's device: the default stream's handle says nothing about its device."""
-        import torch
-        if t.is_cuda and t.device.index != torch.cuda.current_device():
-            return torch.cuda.device(t.device)
-        return contextlib.nullcontext()
+    def call_on(self, t, name, *args):
+        """``call`` with the tensor's device current (the default stream's handle says nothing about its device) and its current
+        stream as the last argument."""
+        if t.is_cuda:
+            import torch
+            if t.device.index != torch.cuda.current_device():
+                with torch.cuda.device(t.device):
+                    return self.call(name, *args, self.stream(t))
+        self.call(name, *args, self.stream(t))
 
     def stream(self, t):
         """Raw handle of the CURRENT stream of the tensor's device (what the reference's ops launch on).  The raw query

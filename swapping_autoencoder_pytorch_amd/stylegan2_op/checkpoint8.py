@@ -47,6 +47,13 @@ class Checkpoint8:
             raise hip_lib.SaeError("Checkpoint8: shape %s is not %d rows of %d" % (tuple(shape), codes.shape[0], channels))
         self.codes, self.scales, self.channels, self.dtype, self.shape = hip_lib.dense(codes), scales, channels, dtype, shape
 
+    @classmethod
+    def _of(cls, codes, scales, channels, dtype, shape):
+        """From parts that are known to fit."""
+        self = object.__new__(cls)
+        self.codes, self.scales, self.channels, self.dtype, self.shape = codes, scales, channels, dtype, shape
+        return self
+
     @property
     def rows(self):
         return self.codes.shape[0]
@@ -59,19 +66,20 @@ class Checkpoint8:
         """The values the codes stand for, a new contiguous tensor."""
         lib = hip_lib.get()
         x = torch.empty(self.shape, dtype=self.dtype, device=self.codes.device)
-        lib.check_channels_last(x)
-        with lib.device_of(x):
-            lib.call("checkpoint8_unpack", self.codes.data_ptr(), self.scales.data_ptr(), x.data_ptr(), self.rows, self.channels,
-                     hip_lib.element_types()[self.dtype], lib.stream(x))
+        code = lib.check_channels_last(x)
+        lib.call_on(x, "checkpoint8_unpack", self.codes.data_ptr(), self.scales.data_ptr(), x.data_ptr(), self.codes.shape[0],
+                    self.channels, code)
         return x
 
 
 def empty_checkpoint8(x):
     """Checkpoint8 of x's type for rows x's leading dimensions, not yet written."""
-    rows, channels = x.shape[:-1].numel(), x.shape[-1]
+    shape = x.shape
+    channels = shape[-1]
+    rows = shape[0] if len(shape) == 2 else shape[:-1].numel()
     blocks = -(-channels // BLOCK)
-    return Checkpoint8(torch.empty(rows, BLOCK * blocks, dtype=torch.int8, device=x.device),
-                       torch.empty(blocks, rows, dtype=torch.uint8, device=x.device), channels, x.dtype, x.shape)
+    return Checkpoint8._of(x.new_empty((rows, BLOCK * blocks), dtype=torch.int8), x.new_empty((blocks, rows), dtype=torch.uint8),
+                           channels, x.dtype, shape)
 
 
 def checkpoint8(x):
@@ -80,12 +88,11 @@ def checkpoint8(x):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise hip_lib.SaeError("checkpoint8: at least one value in the last dimension, got shape %s" % (tuple(x.shape),))
     lib = hip_lib.get()
+    code = lib.check_channels_last(x)
     x = hip_lib.dense(x.detach())
-    lib.check_channels_last(x)
     kept = empty_checkpoint8(x)
-    with lib.device_of(x):
-        lib.call("checkpoint8_pack", x.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), kept.rows, kept.channels,
-                 hip_lib.element_types()[x.dtype], lib.stream(x))
+    lib.call_on(x, "checkpoint8_pack", x.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), kept.codes.shape[0],
+                kept.channels, code)
     return kept
 
 
@@ -94,21 +101,21 @@ def linear_weight_grad8(gy, kept, bias=True, alpha=1.0):
     gw = alpha * gy^T x8, gb = the sum of gy's rows.  In gy's type, which has to be the checkpoint's; the products are exact and
     added in fp32 (f32: gy in three bf16 pieces, which hold all of its 24 bits)."""
     lib = hip_lib.get()
-    if gy.dim() < 1 or gy.shape[-1] < 1 or gy.shape[:-1].numel() != kept.rows:
-        raise hip_lib.SaeError("linear_weight_grad8: gy %s does not have the checkpoint's %d rows" % (tuple(gy.shape), kept.rows))
-    if gy.dtype != kept.dtype or gy.device != kept.codes.device:
+    shape, codes = gy.shape, kept.codes
+    rows, out, c = codes.shape[0], shape[-1] if shape else 0, kept.channels
+    if out < 1 or (shape[0] if len(shape) == 2 else shape[:-1].numel()) != rows:
+        raise hip_lib.SaeError("linear_weight_grad8: gy %s does not have the checkpoint's %d rows" % (tuple(shape), rows))
+    if gy.dtype != kept.dtype or gy.device != codes.device:
         raise hip_lib.SaeError("linear_weight_grad8: gy is %s on %s, the checkpoint %s on %s"
-                               % (gy.dtype, gy.device, kept.dtype, kept.codes.device))
+                               % (gy.dtype, gy.device, kept.dtype, codes.device))
+    code = lib.check_channels_last(gy)
     gy = hip_lib.dense(gy.detach())
-    lib.check_channels_last(gy)
-    out, c = gy.shape[-1], kept.channels
-    gw = torch.empty(out, c, dtype=gy.dtype, device=gy.device)
-    gb = torch.empty(out, dtype=gy.dtype, device=gy.device) if bias else None
-    n_ws = lib.query("linear_wgrad8_workspace", kept.rows, out, c, hip_lib.element_types()[gy.dtype])
-    ws = torch.empty(max(n_ws, 1), dtype=torch.float32, device=gy.device)
-    with lib.device_of(gy):
-        lib.call("linear_wgrad8", gy.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), gw.data_ptr(), hip_lib.ptr(gb),
-                 kept.rows, out, c, float(alpha), hip_lib.element_types()[gy.dtype], ws.data_ptr(), n_ws, lib.stream(gy))
+    gw = gy.new_empty((out, c))
+    gb = gy.new_empty((out,)) if bias else None
+    n_ws = lib.query("linear_wgrad8_workspace", rows, out, c, code)
+    ws = gy.new_empty((n_ws,), dtype=torch.float32) if n_ws else None
+    lib.call_on(gy, "linear_wgrad8", gy.data_ptr(), codes.data_ptr(), kept.scales.data_ptr(), gw.data_ptr(), hip_lib.ptr(gb), rows,
+                out, c, alpha, code, hip_lib.ptr(ws), n_ws)
     return gw, gb
 
 
@@ -132,7 +139,7 @@ class Linear8(Function):
         if ctx.needs_input_grad[0]:
             gx = _gemm(gy, weight, None, False, False, alpha)
         if ctx.needs_input_grad[1] and _Flags.weight_grads:
-            gw, gb = linear_weight_grad8(gy, Checkpoint8(*kept, weight.shape[1], torch.float32), has_bias, alpha)
+            gw, gb = linear_weight_grad8(gy, Checkpoint8._of(*kept, weight.shape[1], torch.float32, None), has_bias, alpha)
         if ctx.needs_input_grad[2] and gb is None:
             gb = gy.sum(0)
         return gx, gw, gb, None, None
@@ -167,8 +174,8 @@ def _pack(t, least):
     k = _Kept()
     k.size, k.stride = t.size(), t.stride()
     n = t.numel()
-    # rows of 4096 values where the memory divides into them: whole blocks either way, the last one alone may be short
-    k.kept = checkpoint8(flat.reshape(-1, 4096) if n % 4096 == 0 else flat.reshape(1, n))
+    # rows of whole blocks where the memory divides into them (else one row, whose last block is short)
+    k.kept = checkpoint8(flat.reshape(-1, next((w for w in (4096, 512, 64, 32) if n % w == 0), n)))
     return k
 
 

@@ -6,55 +6,70 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from .. import hip_lib
-from .checkpoint8 import Checkpoint8, empty_checkpoint8
+from .checkpoint8 import BLOCK
 
 ACTIVATIONS = {"none": 0, "lrelu": 1, "silu": 2}
 
 
+def _last(x):
+    """(dense memory [n, ..., c] of x [n, c, ...], n, positions, c); no copy for a channels-last tensor."""
+    shape = x.shape
+    if len(shape) == 4 and x.is_contiguous(memory_format=torch.channels_last) and x.data_ptr() % 16 == 0:
+        return x, shape[0], shape[2] * shape[3], shape[1]
+    return hip_lib.dense(x.movedim(1, -1)).movedim(-1, 1), shape[0], shape[2:].numel(), shape[1]
+
+
+def _forward(lib, x, weight, bias, groups, eps, act, slope, scale, keep):
+    """(y, x as it is read, stats [2, n, groups], codes, scales)"""
+    code = lib.check_channels_last(x)
+    x, n, l, c = _last(x)
+    y = torch.empty_like(x)                                # (channels last, as x is)
+    stats = x.new_empty((2, n, groups), dtype=torch.float32)
+    codes = scales = None
+    if keep:
+        blocks = -(-c // BLOCK)
+        codes, scales = x.new_empty((n * l, BLOCK * blocks), dtype=torch.int8), x.new_empty((blocks, n * l), dtype=torch.uint8)
+    n_ws = lib.query("group_norm_act_workspace", n, l, c, groups, code, 0)
+    ws = x.new_empty((n_ws,), dtype=torch.uint8) if n_ws else None
+    ptr = hip_lib.ptr
+    mean = stats.data_ptr()
+    lib.call_on(x, "group_norm_act", x.data_ptr(), ptr(weight), ptr(bias), y.data_ptr(), mean, mean + 4 * n * groups, ptr(codes),
+                ptr(scales), n, l, c, groups, eps, act, slope, scale, code, ptr(ws), n_ws)
+    return y, x, stats, codes, scales
+
+
 class GroupNormActFunction(Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, slope, scale, train, keep):
-        lib = hip_lib.get()
-        x = hip_lib.dense(x.movedim(1, -1))                 # [n, ..., c]; no copy for a channels-last tensor
-        weight = None if weight is None else weight.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        lib.check_channels_last(x)
-        n, c = x.shape[0], x.shape[-1]
-        l = x.shape[1:-1].numel()
-        y = torch.empty_like(x)
-        stats = torch.empty(2, n, groups, dtype=torch.float32, device=x.device)
-        kept = empty_checkpoint8(x) if keep else None
-        dt = hip_lib.element_types()[x.dtype]
-        n_ws = lib.query("group_norm_act_workspace", n, l, c, groups, dt, 0)
-        ws = torch.empty(max(n_ws, 1), dtype=torch.uint8, device=x.device)
-        with lib.device_of(x):
-            lib.call("group_norm_act", x.data_ptr(), hip_lib.ptr(weight), hip_lib.ptr(bias), y.data_ptr(), stats[0].data_ptr(),
-                     stats[1].data_ptr(), kept.codes.data_ptr() if keep else None, kept.scales.data_ptr() if keep else None, n, l, c,
-                     groups, eps, act, slope, scale, dt, ws.data_ptr(), n_ws, lib.stream(x))
-        if train:
-            ctx.save_for_backward(weight, bias, stats, *((kept.codes, kept.scales) if keep else (x,)))
-            ctx.cfg = (n, l, c, groups, act, slope, scale, dt)
-        return y.movedim(-1, 1)
+    def forward(ctx, x, weight, bias, groups, eps, act, slope, scale, keep):
+        y, x, stats, codes, scales = _forward(hip_lib.get(), x, weight, bias, groups, eps, act, slope, scale, keep)
+        if keep:
+            ctx.save_for_backward(weight, bias, stats, None, codes, scales)
+        else:
+            ctx.save_for_backward(weight, bias, stats, x, None, None)
+        ctx.cfg = (groups, act, slope, scale)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        weight, bias, stats, *rest = ctx.saved_tensors
-        n, l, c, groups, act, slope, scale, dt = ctx.cfg
+        weight, bias, stats, x, codes, scales = ctx.saved_tensors
+        groups, act, slope, scale = ctx.cfg
         lib = hip_lib.get()
-        gy = hip_lib.dense(gy.movedim(1, -1))
-        lib.check_channels_last(gy)
-        x, codes, scales = (None, *rest) if len(rest) == 2 else (rest[0], None, None)
-        gx = torch.empty_like(gy) if ctx.needs_input_grad[0] else None
-        gw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
-        gb = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
-        n_ws = lib.query("group_norm_act_workspace", n, l, c, groups, dt, 1)
-        ws = torch.empty(max(n_ws, 1), dtype=torch.uint8, device=gy.device)
-        with lib.device_of(gy):
-            lib.call("group_norm_act_bwd", gy.data_ptr(), hip_lib.ptr(x), hip_lib.ptr(codes), hip_lib.ptr(scales),
-                     stats[0].data_ptr(), stats[1].data_ptr(), hip_lib.ptr(weight), hip_lib.ptr(bias), hip_lib.ptr(gx),
-                     hip_lib.ptr(gw), hip_lib.ptr(gb), n, l, c, groups, act, slope, scale, dt, ws.data_ptr(), n_ws, lib.stream(gy))
-        return None if gx is None else gx.movedim(-1, 1), gw, gb, None, None, None, None, None, None, None
+        code = lib.check_channels_last(gy)
+        if x is not None:
+            x = _last(x)[0]
+        gy, n, l, c = _last(gy)
+        need = ctx.needs_input_grad
+        gx = torch.empty_like(gy) if need[0] else None
+        gw = torch.empty_like(weight) if need[1] else None
+        gb = torch.empty_like(bias) if need[2] else None
+        n_ws = lib.query("group_norm_act_workspace", n, l, c, groups, code, 1)
+        ws = gy.new_empty((n_ws,), dtype=torch.uint8) if n_ws else None
+        ptr = hip_lib.ptr
+        mean = stats.data_ptr()
+        lib.call_on(gy, "group_norm_act_bwd", gy.data_ptr(), ptr(x), ptr(codes), ptr(scales), mean, mean + 4 * n * groups,
+                    ptr(weight), ptr(bias), ptr(gx), ptr(gw), ptr(gb), n, l, c, groups, act, slope, scale, code, ptr(ws), n_ws)
+        return gx, gw, gb, None, None, None, None, None, None
 
 
 def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, activation="lrelu", negative_slope=0.2, scale=None,
@@ -73,16 +88,20 @@ def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, activati
         raise hip_lib.SaeError("group_norm_act: x must be [N, C, ...] with C a multiple of num_groups = %d, got %s"
                                % (num_groups, tuple(input.shape)))
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (input.shape[1],) or t.device != input.device):
+        if t is not None and (t.dtype != torch.float32 or t.shape != input.shape[1:2] or t.device != input.device):
             raise hip_lib.SaeError("group_norm_act: %s must be float32 [%d] on %s, got %s %s on %s"
                                    % (name, input.shape[1], input.device, t.dtype, tuple(t.shape), t.device))
     if not eps >= 0:
         raise hip_lib.SaeError("group_norm_act: eps must not be negative, got %r" % (eps,))
     if scale is None:
         scale = 2 ** 0.5 if activation == "lrelu" else 1.0
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, bias))
-    return GroupNormActFunction.apply(input, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation],
-                                      float(negative_slope), float(scale), train, bool(checkpoint) and train)
+    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    if torch.is_grad_enabled() and (input.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return GroupNormActFunction.apply(input, weight, bias, num_groups, eps, ACTIVATIONS[activation], negative_slope, scale,
+                                          bool(checkpoint))
+    return _forward(hip_lib.get(), input, weight, bias, num_groups, eps, ACTIVATIONS[activation], negative_slope, scale, False)[0]
 
 
 class GroupNormAct(nn.Module):
