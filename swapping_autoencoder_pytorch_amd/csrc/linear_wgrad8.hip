@@ -84,46 +84,42 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base, int6
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
 }
 
-// A thread's 4 rows x 4 channels of gy, as loaded
-template <int DT, bool VEC>
-struct GyQuad {
+// A thread's 4 rows x CH channels of gy, as loaded: 16 bytes of each row (4 or 8 channels), at dword addresses.  Where a row ends inside
+// them, the channels behind its end are whatever follows; they only meet outputs that are not there.  ODD: 16-bit rows of odd length,
+// every other one of which starts in the middle of a dword -- rows 1 and 3: five dwords from half a dword in front.
+template <int DT, bool ODD>
+struct GyBox {
     using T = typename Elem<DT>::T;
-    float f[4][4];     // f32
-    u32x2 h[4];        // 16-bit types: 4 channels of a row
-    // row i: r0 + mine + i of a slice of `rows` (r0 the same in a wave, mine not), channels o ... o + 3 of it.
-    // VEC: the quad is there or not (out % 4 == 0); mine and o are in the lane's offset `at`, r0 in the scalar one, which stays
-    // within the descriptor
-    __device__ __forceinline__ void load(int i, __amdgpu_buffer_rsrc_t all, unsigned at, const T* __restrict__ gy, int r0, int mine,
-                                         int rows, int o, int out) {
-        if constexpr (VEC) {
-            const unsigned from = (unsigned)(r0 + i < rows ? r0 + i : rows) * (unsigned)out * (unsigned)sizeof(T);
-            if constexpr (DT == SAE_F32) {
-                const u32x4 q = __builtin_amdgcn_raw_buffer_load_b128(all, at, from, 0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f[i][j] = bits_f(q[j]);
-            } else {
-                h[i] = __builtin_amdgcn_raw_buffer_load_b64(all, at, from, 0);
-            }
+    static constexpr int CH = 16 / (int)sizeof(T);
+    u32x4 q[4];
+    unsigned fifth[2]; // of rows 1 and 3
+    // row i: r0 + mine + i of a slice of `rows` (r0, the same in a wave, is in the scalar offset, which stays within the descriptor;
+    // mine, a multiple of four, and the channel are in the lane's offset `at`)
+    __device__ __forceinline__ void load(int i, __amdgpu_buffer_rsrc_t all, unsigned at, int r0, int rows, int out) {
+        const bool on = r0 + i < rows;
+        const unsigned from = (unsigned)(on ? r0 + i : rows) * (unsigned)out * (unsigned)sizeof(T);
+        if (ODD && (i & 1)) {
+            const unsigned whole = on ? from - 2u : (from + 3u) & ~3u;
+            q[i] = __builtin_amdgcn_raw_buffer_load_b128(all, at, whole, 0);
+            fifth[i >> 1] = __builtin_amdgcn_raw_buffer_load_b32(all, at + 16u, whole, 0);
         } else {
-            const bool on = r0 + mine + i < rows;
-            const T* p = gy + (int64_t)(r0 + mine + i) * out + o;
-            unsigned v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const T e = on && o + j < out ? p[j] : (T)0;
-                if constexpr (DT == SAE_F32) f[i][j] = e;
-                else v[j] = e;
-            }
-            if constexpr (DT != SAE_F32) h[i] = u32x2{v[0] | (v[1] << 16), v[2] | (v[3] << 16)};
+            q[i] = __builtin_amdgcn_raw_buffer_load_b128(all, at, ODD ? (from + 3u) & ~3u : from, 0);
         }
     }
-    // channel j of rows i and i + 1, as a word (16-bit types)
-    __device__ __forceinline__ unsigned pair(int i, int j) const {
-        return j & 1 ? halves<true>(h[i][j >> 1], h[i + 1][j >> 1]) : halves<false>(h[i][j >> 1], h[i + 1][j >> 1]);
+    __device__ __forceinline__ float value(int i, int j) const { return bits_f(q[i][j]); }      // (f32)
+    // channels 2 k and 2 k + 1 of row i (16-bit types); have: rows that are there (ODD: half a dword behind the last one is not)
+    __device__ __forceinline__ unsigned word(int i, int k, int have) const {
+        unsigned w = q[i][k];
+        if constexpr (ODD) {
+            if (i & 1) w = (w >> 16) | ((k < 3 ? q[i][(k + 1) & 3] : fifth[i >> 1]) << 16);
+            if (i >= have) w = 0u;
+        }
+        return w;
     }
-    __device__ __forceinline__ float value(int i, int j) const {
-        if constexpr (DT == SAE_F32) return f[i][j];
-        else return widen<DT>((uint16_t)(h[i][j >> 1] >> (16 * (j & 1))));
+    // channel j of rows i and i + 1, as a word
+    __device__ __forceinline__ unsigned pair(int i, int j, int have) const {
+        const unsigned a = word(i, j >> 1, have), b = word(i + 1, j >> 1, have);
+        return j & 1 ? halves<true>(a, b) : halves<false>(a, b);
     }
 };
 
@@ -138,30 +134,31 @@ __device__ __forceinline__ float rest8(float v) {
 template <int DT, int BM>
 struct WgTile {
     static constexpr int PL = DT == SAE_F32 ? 3 : 1;              // pieces of gy
-    static constexpr int KR = DT == SAE_F32 ? 32 : 64;            // rows of a step: 2 x 56 / 2 x 48 KB of LDS at BM = 256
+    static constexpr int KR = DT == SAE_F32 ? 32 : 64;            // rows of a step: 2 x 56 KB (f32, BM 256), 2 x 32 KB (others, 128) of LDS
     static constexpr int OCT = KR / 8;
-    static constexpr int AQ = BM / 4 * (KR / 4);                  // gy quads of a step
+    static constexpr int CH = DT == SAE_F32 ? 4 : 8;              // channels of gy of a thread's box (4 rows of them: GyBox)
+    static constexpr int AQ = BM / CH * (KR / 4);                 // boxes of a step
     static constexpr int NA = AQ / kBlock > 0 ? AQ / kBlock : 1;  // of a thread
-    static constexpr int AR = kBlock / (BM / 4);                  // row quads that the threads cover at once
+    static constexpr int AR = kBlock / (BM / CH);                 // row quads that the threads cover at once
     static constexpr int NB = kBN / 4 * (KR / 4) / kBlock;        // codes quads of a thread
     static constexpr int WM = BM == 256 ? 2 : 1;                  // 32-channel tiles of a wave: 64 x 128 (BM 256),
     static constexpr int WN = BM == 64 ? 2 : 4;                   // 32 x 128 (128), 32 x 64 (64)
     static constexpr int CELLS = OCT * (PL * BM + kBN);           // 16-byte cells of a step
-    // position of channel 4 q + j: groups of 128 channels, 32 j + q inside (BM = 64: 16 j + q)
-    static __device__ __forceinline__ int place(int q, int j) { return BM == 64 ? 16 * j + q : (q >> 5) * 128 + 32 * j + (q & 31); }
-    static __device__ __forceinline__ int channel(int at) {
-        return BM == 64 ? 4 * (at & 15) + (at >> 4) : (at >> 7) * 128 + 4 * (at & 31) + ((at >> 5) & 3);
-    }
+    // position of channel CH q + j of gy: groups of 128 channels, G j + q inside; and the channel of a position
+    static constexpr int G = (BM < 128 ? BM : 128) / CH;
+    static __device__ __forceinline__ int place(int q, int j) { return q / G * 128 + G * j + q % G; }
+    static __device__ __forceinline__ int channel(int at) { return (at >> 7) * 128 + CH * (at % G) + (at & 127) / G; }
 };
 
-template <int DT, int BM, bool VEC, bool WHOLE>
+template <int DT, int BM, bool ODD, bool WHOLE>
 __global__ __launch_bounds__(kBlock, BM == 256 ? 1 : 2)
 void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int8_t* __restrict__ codes,
                           const uint8_t* __restrict__ scales, float* __restrict__ part, float* __restrict__ part_b,
                           typename Elem<DT>::T* __restrict__ gw, typename Elem<DT>::T* __restrict__ gb, float alpha, const WgShape p) {
     using W = WgTile<DT, BM>;
     using T = typename Elem<DT>::T;
-    constexpr int PL = W::PL, KR = W::KR, OCT = W::OCT, NA = W::NA, NB = W::NB, WM = W::WM, WN = W::WN, AR = W::AR;
+    constexpr int PL = W::PL, KR = W::KR, OCT = W::OCT, NA = W::NA, NB = W::NB, WM = W::WM, WN = W::WN, AR = W::AR,
+                  CH = W::CH;
     __shared__ u32x4 cells[2][W::CELLS];                          // of a step: gy [PL][OCT][BM], codes [OCT][kBN]
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -179,29 +176,29 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
     const int64_t ld = (int64_t)p.blocks * kBlk8;
 
     f32x16 acc[WM][WN];
-    float sum[4];                                                 // gb: the thread's channels are the same in every step
+    float sum[2 * CH];                                            // gb (the thread's channels are the same in every step), in two shares
+    float pace[NB][4];                                            // steps 2^k of the codes' rows
 
     // what a step's loads bring a thread; two steps are under way
     struct Load {
-        GyQuad<DT, VEC> g[NA];
+        GyBox<DT, ODD> g[NA];
         unsigned cw[NB][4], ce[NB];
     };
     Load load[2];
     // neighbouring lanes take the two row quads of a cell: their 8-byte writes fill whole cells, without a bank conflict
-    const int oq = (tid >> 1) % (BM / 4), ar = (tid & 1) + 2 * (tid / (BM / 2));   // gy: channel quad, row quad (of every AR)
-    const int bq = (tid >> 1) & 31, br = (tid & 1) + 2 * (tid >> 6);               // codes: channel quad, row quad (of every 8)
+    const int oq = (tid >> 1) % (BM / CH), ar = (tid & 1) + 2 * (tid / (2 * BM / CH));   // gy: channels, row quad (of every AR)
+    const int bq = (tid >> 1) & 31, br = (tid & 1) + 2 * (tid >> 6);                     // codes: channel quad, row quad (of every 8)
     const bool a_in = W::AQ >= kBlock || ar < KR / 4, b_in = i0 + 4 * bq < ld;
-    const T* const gsrc = gy + r_begin * p.out;
-    const __amdgpu_buffer_rsrc_t grows = rows_of(gsrc, (int64_t)rows * p.out * (int64_t)sizeof(T));
+    const __amdgpu_buffer_rsrc_t grows = rows_of(gy + r_begin * p.out, ((int64_t)rows * p.out * (int64_t)sizeof(T) + 3) & ~(int64_t)3);
     const __amdgpu_buffer_rsrc_t crows = rows_of(codes + r_begin * ld, rows * ld);
     const uint8_t* const ssrc = scales + (int64_t)(b_in ? (i0 + 4 * bq) / kBlk8 : 0) * p.rows + r_begin;
     const unsigned nowhere = 0xfffffff0u;                         // behind every descriptor
-    const unsigned gat = a_in && o0 + 4 * oq < p.out
-                             ? ((unsigned)(4 * ar) * (unsigned)p.out + (unsigned)(o0 + 4 * oq)) * (unsigned)sizeof(T) : nowhere;
+    const unsigned gat = a_in && o0 + CH * oq < p.out
+                             ? ((unsigned)(4 * ar) * (unsigned)p.out + (unsigned)(o0 + CH * oq)) * (unsigned)sizeof(T) : nowhere;
     const unsigned cat = b_in ? (unsigned)(4 * br) * (unsigned)ld + (unsigned)(i0 + 4 * bq) : nowhere;
 
-    auto fetch_gy = [&](Load& to, int step, int n) {              // n < 4 NA: one row of a quad
-        to.g[n >> 2].load(n & 3, grows, gat, gsrc, step * KR + 4 * AR * (n >> 2), 4 * ar, a_in ? rows : 0, o0 + 4 * oq, p.out);
+    auto fetch_gy = [&](Load& to, int step, int n) {              // n < 4 NA: one row of a box
+        to.g[n >> 2].load(n & 3, grows, gat, step * KR + 4 * AR * (n >> 2), rows, p.out);
     };
     auto fetch_codes = [&](Load& to, int step, int n) {           // n < 5 NB: four rows of a quad, and their exponents
         const int q = n / 5, i = n % 5;
@@ -227,18 +224,18 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
             for (int n = 0; n < 5 * NB; ++n) fetch_codes(to, step, n);
     };
     auto put = [&](u32x4* cell, int rq, unsigned lo, unsigned hi) { *(reinterpret_cast<u32x2*>(cell) + (rq & 1)) = u32x2{lo, hi}; };
-    // One channel of a quad: of gy (n < 4 NA) or of the codes.  ODD: with infinities and NaN among the values (f32)
-    constexpr int PIECES = 4 * (NA + NB);
+    // One channel of a box: of gy (n < CH NA) or of the codes.  odd: with infinities and NaN among the values (f32)
+    constexpr int PIECES = CH * NA + 4 * NB;
     auto stage = [&](const Load& from, int step, u32x4* to, int n, auto odd) {
-        if (n < 4 * NA) {
-            const int q = n >> 2, j = n & 3, rq = ar + AR * q;
+        if (n < CH * NA) {
+            const int q = n / CH, j = n % CH, rq = ar + AR * q;
             u32x4* const row = to + (rq >> 1) * BM + W::place(oq, j);
             if constexpr (DT == SAE_F32) {
                 float v[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    v[i] = from.g[q].f[i][j];
-                    sum[j] += v[i];
+                    v[i] = from.g[q].value(i, j);
+                    sum[(i & 1) * CH + j] += v[i];
                     if (odd.value && v[i] != v[i]) v[i] = bits_f(0x7fc00000u);       // (a NaN of low bits alone is cut to infinity)
                 }
 #pragma unroll
@@ -249,17 +246,24 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
                     for (int i = 0; i < 4; ++i) v[i] = rest8<odd.value>(v[i]);
                 }
             } else {
-                const unsigned lo = from.g[q].pair(0, j), hi = from.g[q].pair(2, j);
-                sum[j] = add_pair<DT>(add_pair<DT>(sum[j], lo), hi);
+                const int have = rows - (step * KR + 4 * rq);
+                const unsigned lo = from.g[q].pair(0, j, have), hi = from.g[q].pair(2, j, have);
+                sum[j] = add_pair<DT>(sum[j], lo);
+                sum[CH + j] = add_pair<DT>(sum[CH + j], hi);
                 if (W::AQ >= kBlock || rq < KR / 4) put(row, rq, lo, hi);
             }
         } else {
-            const int q = (n >> 2) - NA, j = n & 3, rq = br + 8 * q, r = step * KR + 4 * rq;
-            const int by = r < last ? 0 : r - last, have = rows - r;    // the word shifted, and cut to the slice's rows
-            const unsigned e = have <= 0 ? 0u : (from.ce[q] >> (8 * by)) & (have >= 4 ? 0xffffffffu : (1u << (8 * have)) - 1u);
+            const int m = n - CH * NA, q = m >> 2, j = m & 3, rq = br + 8 * q;
+            if (j == 0) {                                         // the word of exponents shifted, and cut to the slice's rows
+                const int r = step * KR + 4 * rq, by = r > last ? r - last : 0;
+                const int have = rows - r < 0 ? 0 : rows - r < 4 ? rows - r : 4;
+                const unsigned e = (from.ce[q] >> (8 * (by & 3))) & (unsigned)(((uint64_t)1 << (8 * have)) - 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pace[q][i] = block8_step((e >> (8 * i)) & 0xffu);
+            }
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(from.cw[q][i] >> (8 * j)) * block8_step((e >> (8 * i)) & 0xffu);
+            for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(from.cw[q][i] >> (8 * j)) * pace[q][i];
             put(to + PL * OCT * BM + (rq >> 1) * kBN + 32 * j + bq, rq, pack_exact<DT>(v[0], v[1]), pack_exact<DT>(v[2], v[3]));
         }
     };
@@ -308,7 +312,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[m][n][r] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] = 0.0f;
+        for (int j = 0; j < 2 * CH; ++j) sum[j] = 0.0f;
     };
 
     clear();
@@ -331,8 +335,8 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
                 if (n < 5 * NB) {
                     fetch_codes(before, step + 2, n);
                 } else {
-                    const int m = n - 5 * NB;                     // (its quad is staged by then)
-                    static_assert(5 * NB * PARTS / LOADS >= 3 * PARTS / PIECES && (LOADS - 4) * PARTS / LOADS >= (4 * NA - 1) * PARTS / PIECES, "order");
+                    const int m = n - 5 * NB;                     // (its box is staged by then)
+                    static_assert(5 * NB * PARTS / LOADS >= (CH - 1) * PARTS / PIECES && (LOADS - 4) * PARTS / LOADS >= (CH * NA - 1) * PARTS / PIECES, "order");
                     fetch_gy(next, step + 3, m);
                 }
             }
@@ -399,7 +403,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
         float* const fold = reinterpret_cast<float*>(&cells[0][0]);
         if (ar < AG)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) fold[ar * BM + 4 * oq + j] = sum[j];
+            for (int j = 0; j < CH; ++j) fold[ar * BM + CH * oq + j] = sum[j] + sum[CH + j];
         __syncthreads();
         for (int o = tid; o < BM; o += kBlock) {
             float t = fold[o];
@@ -465,15 +469,19 @@ struct WgPlan {
     WgShape p;
 };
 
-// The tallest tile that still gives every CU a work-group of at least two steps a wave group, 64 if none does; slices so that the
-// work-groups fill the 256 CUs in as few rounds as the work allows.
+// Tiles of 256 channels of gy and one work-group a CU in f32, whose three pieces fill the matrix cores from one wave a SIMD; of 128 and
+// two work-groups a CU in the 16-bit types, where reading operands takes longer than multiplying them (bf16 65536 x 512 x 512: 63 us
+// so, 68 with the tall tile; f32 16384 x 1024 x 2048: 209 either way).  Shorter ones where those would leave CUs without a work-group
+// of four steps.  Slices so that the work-groups fill the chip once.
 WgPlan wg_plan(int64_t rows, int64_t out, int64_t c, int32_t dtype) {
     const int kr = wg_rows(dtype);
     const int64_t steps = ceil_div64(rows, kr), pairs = ceil_div64(steps, 4), tiles_n = ceil_div64(c, kBN);
     int bm = 64;
-    for (int t : {256, 128})
+    for (int t = dtype == SAE_F32 ? 256 : 128; t > 64; t /= 2)
         if (out > t / 2 && ceil_div64(out, t) * tiles_n * pairs >= 256) { bm = t; break; }
-    if (const int forced = tuning_knob("SAE_WG_TILE", 0)) bm = forced;      // (tests: every height at small sizes)
+    const int forced = tuning_knob("SAE_WG_TILE", 0);                       // (tests: every height at small sizes)
+    if (forced && (forced <= 128 || dtype == SAE_F32)) bm = forced;
+    const int64_t full = bm == 256 ? 256 : 512;
     WgPlan w;
     w.bm = bm;
     w.p.rows = rows;
@@ -484,9 +492,9 @@ WgPlan wg_plan(int64_t rows, int64_t out, int64_t c, int32_t dtype) {
     w.p.tiles_n = (int)tiles_n;
     const int64_t tiles = ceil_div64(out, bm) * tiles_n;
     int64_t best = 1;
-    if (tiles < 256) {
-        best = 256 / tiles;
-        if (best > 8) best = best / 8 * 8;
+    if (tiles < full) {
+        best = full / tiles;
+        if (best > 8) best = best / 8 * 8;                                  // (whole slices on each of the eight XCDs)
     }
     if (best > pairs) best = pairs;
     // a slice's rows lie behind one descriptor with 32-bit offsets
@@ -507,16 +515,16 @@ bool wg_shape_ok(int64_t rows, int64_t out, int64_t c) {
            rows <= ((int64_t)1 << 40) / (out + c);
 }
 
-template <int DT, int BM, bool VEC>
+template <int DT, int BM, bool ODD>
 void wg_launch(const void* gy, const int8_t* codes, const uint8_t* scales, float* part, float* part_b, void* gw, void* gb, float alpha,
                const WgShape& p, hipStream_t s) {
     using T = typename Elem<DT>::T;
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n * p.slices)), block(kBlock);
     if (p.slices == 1)
-        hipLaunchKernelGGL((linear_wgrad8_kernel<DT, BM, VEC, true>), grid, block, 0, s, (const T*)gy, codes, scales, part, part_b,
+        hipLaunchKernelGGL((linear_wgrad8_kernel<DT, BM, ODD, true>), grid, block, 0, s, (const T*)gy, codes, scales, part, part_b,
                            (T*)gw, (T*)gb, alpha, p);
     else
-        hipLaunchKernelGGL((linear_wgrad8_kernel<DT, BM, VEC, false>), grid, block, 0, s, (const T*)gy, codes, scales, part, part_b,
+        hipLaunchKernelGGL((linear_wgrad8_kernel<DT, BM, ODD, false>), grid, block, 0, s, (const T*)gy, codes, scales, part, part_b,
                            (T*)gw, (T*)gb, alpha, p);
 }
 
@@ -531,14 +539,14 @@ int wg_run(const void* gy, const int8_t* codes, const uint8_t* scales, void* gw,
     }
     const WgPlan w = wg_plan(rows, out, c, DT);
     const WgShape& p = w.p;
-    const bool vec = out % 4 == 0 && reinterpret_cast<uintptr_t>(gy) % (4 * sizeof(T)) == 0;
     float* part_b = gb ? ws + (int64_t)p.slices * out * p.blocks * kBlk8 : nullptr;
 #define SAE_WG(BM)                                                                                                              \
-    if (vec) wg_launch<DT, BM, true>(gy, codes, scales, ws, part_b, gw, gb, alpha, p, s);                                       \
+    if (DT != SAE_F32 && out % 2 != 0)                                                                                          \
+        wg_launch<DT, BM, DT != SAE_F32>(gy, codes, scales, ws, part_b, gw, gb, alpha, p, s);                                   \
     else wg_launch<DT, BM, false>(gy, codes, scales, ws, part_b, gw, gb, alpha, p, s)
     if (w.bm == 64) { SAE_WG(64); }
     else if (w.bm == 128) { SAE_WG(128); }
-    else { SAE_WG(256); }
+    else if constexpr (DT == SAE_F32) { SAE_WG(256); }
 #undef SAE_WG
     if (p.slices > 1)
         hipLaunchKernelGGL((linear_wgrad8_reduce_kernel<DT>), dim3((unsigned)ceil_div64(out * p.blocks * kBlk8, 256)),
@@ -563,7 +571,7 @@ extern "C" int sae_linear_wgrad8(const void* gy, const int8_t* codes, const uint
     if (!elem_known(dtype)) return fail(SAE_EINVAL, "sae_linear_wgrad8: unknown element type %d", (int)dtype);
     if (!wg_shape_ok(rows, out, c)) return fail(SAE_EINVAL, "sae_linear_wgrad8: bad shape");
     if (!gw || (rows > 0 && (!gy || !codes || !scales))) return fail(SAE_EINVAL, "sae_linear_wgrad8: null tensor");
-    if (rows > 0 && (!aligned16(codes) || !aligned16(workspace) || reinterpret_cast<uintptr_t>(gy) % (uintptr_t)elem_bytes(dtype)))
+    if (rows > 0 && (!aligned16(codes) || !aligned16(workspace) || !aligned16(gy)))
         return fail(SAE_EINVAL, "sae_linear_wgrad8: misaligned tensor");
     const int64_t need = sae_linear_wgrad8_workspace(rows, out, c, dtype);
     if (need > 0 && (!workspace || workspace_floats < need))
