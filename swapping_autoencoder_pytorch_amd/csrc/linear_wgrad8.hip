@@ -393,8 +393,11 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
                 }
             } else if (i < ld) {
                 float* const dst = part + ((int64_t)slice * p.out + o) * ld + i;
-                if constexpr (WN == 4) *reinterpret_cast<f32x4*>(dst) = f32x4{acc[m][0][r], acc[m][1][r], acc[m][2][r], acc[m][3][r]};
-                else *reinterpret_cast<f32x2*>(dst) = f32x2{acc[m][0][r], acc[m][1][r]};
+                // (past the caches, written once and read once: 67 -> 64 us on bf16 65536 x 512 x 512)
+                if constexpr (WN == 4)
+                    __builtin_nontemporal_store(f32x4{acc[m][0][r], acc[m][1][r], acc[m][2][r], acc[m][3][r]}, reinterpret_cast<f32x4*>(dst));
+                else
+                    __builtin_nontemporal_store(f32x2{acc[m][0][r], acc[m][1][r]}, reinterpret_cast<f32x2*>(dst));
             }
         }
     }
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(kBlock) void linear_wgrad8_reduce_kernel(const floa
     if (e < size)
 #pragma unroll 8
         for (int s = first; s < end; ++s) {
-            const f32x4 t = *reinterpret_cast<const f32x4*>(part + s * size + e);
+            const f32x4 t = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(part + s * size + e));
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] += t[j];
         }
