@@ -9,18 +9,23 @@
 // v_mfma_f32_32x32x16 at 3 products has five times the rate of v_mfma_f32_32x32x2_f32: keeping x in 8 bits makes the f32 weight
 // gradient faster than the exact f32 product of the full-width tensors, not only smaller.
 //
-// Tile: BM channels of gy x 128 channels of x, 32 rows (f32) or 64 at a time, four waves.  The sum runs over ROWS, the slow axis of
-// both tensors, while a matrix-core operand wants 8 rows of one channel next to each other: a thread loads 4 channels of 4 rows (16
-// bytes a row of f32 gy, 4 bytes a row of codes), and writes for each of its 4 channels the 4 rows packed to 8 bytes.  LDS holds
-// 16-byte cells [k octet][position], where channel 4 j + m of a group of 128 sits at position 32 m + j: lanes that stage neighbouring
-// quads write neighbouring cells, an operand is one 16-byte read with neighbouring lanes on neighbouring cells (no bank conflict, by
-// the counters), and a lane ends up with the 4 neighbouring output channels 4 j ... 4 j + 3 in its 4 accumulators -- whole 16-byte
+// Tile: BM channels of gy x 128 channels of x, 32 rows (f32) or 64 at a time; 256 x 128 in eight waves of 64 x 128, each group of four
+// with half of a step's rows, where there is work for it, 128 and 64 in four waves where not.  The sum runs over ROWS, the slow axis of
+// both tensors, while a matrix-core operand wants 8 rows of one channel next to each other: a thread loads 16 bytes (4 or 8 channels) of
+// 4 rows of gy and 4 codes of 4 rows, and writes for each of its channels the 4 rows packed to 8 bytes.  LDS holds 16-byte cells
+// [k octet][position], where the j-th channel of the q-th thread sits at G j + q of its group of 128: lanes that stage neighbouring
+// channels write neighbouring cells, and an operand is one 16-byte read with neighbouring lanes on neighbouring cells (no bank conflict,
+// by the counters).  For the codes G = 32, and a lane ends up with 4 neighbouring output channels in its 4 accumulators: whole 16-byte
 // stores, no shuffle.
 //
 // What bounds it: a wave issues in order, so everything a step needs beside its products -- cutting gy, decoding codes, LDS writes,
-// the loads two steps ahead -- is dealt out between them (`multiply`).  Measured on f32 16384 x 1024 x 2048: 340 us with one set of
-// cells and a burst of each; 229 us with two groups of four waves that stage and multiply in turn (their loads, one step ahead, are
-// waited for); 206 us in this form, of which the products alone take 140.  bf16 65536 x 512 x 512: 140 -> 77 us.
+// the loads two steps ahead -- is dealt out between them (`multiply`).  Measured (f32 16384 x 1024 x 2048, bf16 65536 x 512 x 512):
+//     340, 140 us   one set of cells, a burst of loads, then of vector work, then of products
+//     229, 100      two groups of four waves that stage and multiply in turn; their loads, one step ahead, are waited for
+//     207, 65       four waves, dealt out; operands read ahead
+//     205, 58       eight waves (this form): two on a SIMD to cover each other
+// f32: 1010 - 1040 TFLOP/s on the matrix cores (a library's bf16 product of 8192^3 reaches 1217 on this card; with gy = 0 the same
+// launch takes 177 us: the clock).  bf16: 44 us here and 12 in the kernel that adds the slices; at 65536 x 1024 x 2048 870 TFLOP/s.
 //
 // Few tiles: the rows are cut into slices, one work-group each, whose fp32 tiles a second kernel adds in order.
 #include "elem8.inc"
@@ -134,13 +139,17 @@ __device__ __forceinline__ float rest8(float v) {
 template <int DT, int BM>
 struct WgTile {
     static constexpr int PL = DT == SAE_F32 ? 3 : 1;              // pieces of gy
-    static constexpr int KR = DT == SAE_F32 ? 32 : 64;            // rows of a step: 2 x 56 KB (f32, BM 256), 2 x 32 KB (others, 128) of LDS
+    static constexpr int KR = DT == SAE_F32 ? 32 : 64;            // rows of a step: 2 x 56 (f32) or 2 x 48 KB of LDS at BM = 256
     static constexpr int OCT = KR / 8;
+    static constexpr int GROUPS = BM == 256 ? 2 : 1;              // of four waves, each with a share of a step's rows: two waves a SIMD
+    static constexpr int T = 256 * GROUPS;                        // threads
     static constexpr int CH = DT == SAE_F32 ? 4 : 8;              // channels of gy of a thread's box (4 rows of them: GyBox)
     static constexpr int AQ = BM / CH * (KR / 4);                 // boxes of a step
-    static constexpr int NA = AQ / kBlock > 0 ? AQ / kBlock : 1;  // of a thread
-    static constexpr int AR = kBlock / (BM / CH);                 // row quads that the threads cover at once
-    static constexpr int NB = kBN / 4 * (KR / 4) / kBlock;        // codes quads of a thread
+    static constexpr int NA = AQ / T > 0 ? AQ / T : 1;            // of a thread
+    static constexpr int AR = T / (BM / CH);                      // row quads that the threads cover at once
+    static constexpr int BQ = kBN / 4 * (KR / 4);                 // codes quads of a step
+    static constexpr int NB = BQ / T > 0 ? BQ / T : 1;            // of a thread
+    static constexpr int BR = (T < BQ ? T : BQ) / 32;             // row quads of codes at once
     static constexpr int WM = BM == 256 ? 2 : 1;                  // 32-channel tiles of a wave: 64 x 128 (BM 256),
     static constexpr int WN = BM == 64 ? 2 : 4;                   // 32 x 128 (128), 32 x 64 (64)
     static constexpr int CELLS = OCT * (PL * BM + kBN);           // 16-byte cells of a step
@@ -151,17 +160,17 @@ struct WgTile {
 };
 
 template <int DT, int BM, bool ODD, bool WHOLE>
-__global__ __launch_bounds__(kBlock, BM == 256 ? 1 : 2)
+__global__ __launch_bounds__((WgTile<DT, BM>::T), 2)
 void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int8_t* __restrict__ codes,
                           const uint8_t* __restrict__ scales, float* __restrict__ part, float* __restrict__ part_b,
                           typename Elem<DT>::T* __restrict__ gw, typename Elem<DT>::T* __restrict__ gb, float alpha, const WgShape p) {
     using W = WgTile<DT, BM>;
     using T = typename Elem<DT>::T;
     constexpr int PL = W::PL, KR = W::KR, OCT = W::OCT, NA = W::NA, NB = W::NB, WM = W::WM, WN = W::WN, AR = W::AR,
-                  CH = W::CH;
+                  CH = W::CH, BR = W::BR, GROUPS = W::GROUPS;
     __shared__ u32x4 cells[2][W::CELLS];                          // of a step: gy [PL][OCT][BM], codes [OCT][kBN]
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
-    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wid = wave & 3, group = wave >> 2;
     // Work-groups go round the eight XCDs.  Each XCD takes a run of neighbouring (slice, tile row, tile column): whole slices where
     // there are eight or more, else tile rows of one, so that its L2 reads a tile of gy once for all the columns beside it.
     const int tiles = p.tiles_m * p.tiles_n, all = (int)gridDim.x, xcd = blockIdx.x & 7;
@@ -187,8 +196,9 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
     Load load[2];
     // neighbouring lanes take the two row quads of a cell: their 8-byte writes fill whole cells, without a bank conflict
     const int oq = (tid >> 1) % (BM / CH), ar = (tid & 1) + 2 * (tid / (2 * BM / CH));   // gy: channels, row quad (of every AR)
-    const int bq = (tid >> 1) & 31, br = (tid & 1) + 2 * (tid >> 6);                     // codes: channel quad, row quad (of every 8)
-    const bool a_in = W::AQ >= kBlock || ar < KR / 4, b_in = i0 + 4 * bq < ld;
+    const int bt = tid % (32 * BR);                              // (more threads than quads: the second half stages the same again)
+    const int bq = (bt >> 1) & 31, br = (bt & 1) + 2 * (bt >> 6);                        // codes: channel quad, row quad (of every BR)
+    const bool a_in = W::AQ >= W::T || ar < KR / 4, b_in = i0 + 4 * bq < ld;
     const __amdgpu_buffer_rsrc_t grows = rows_of(gy + r_begin * p.out, ((int64_t)rows * p.out * (int64_t)sizeof(T) + 3) & ~(int64_t)3);
     const __amdgpu_buffer_rsrc_t crows = rows_of(codes + r_begin * ld, rows * ld);
     const uint8_t* const ssrc = scales + (int64_t)(b_in ? (i0 + 4 * bq) / kBlk8 : 0) * p.rows + r_begin;
@@ -203,11 +213,11 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
     auto fetch_codes = [&](Load& to, int step, int n) {           // n < 5 NB: four rows of a quad, and their exponents
         const int q = n / 5, i = n % 5;
         if (i < 4) {
-            const int from = step * KR + 32 * q + i;
+            const int from = step * KR + 4 * BR * q + i;
             to.cw[q][i] = __builtin_amdgcn_raw_buffer_load_b32(crows, cat, (unsigned)(from < rows ? from : rows) * (unsigned)ld, 0);
             return;
         }
-        const int r = step * KR + 4 * (br + 8 * q);
+        const int r = step * KR + 4 * (br + BR * q);
         if (p.rows >= 4) {                                        // a word that ends at the block's last row at most
             __builtin_memcpy(&to.ce[q], ssrc + (r < last ? r : last), 4);
         } else {
@@ -240,7 +250,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
                 }
 #pragma unroll
                 for (int s = 0; s < 3; ++s) {
-                    if (W::AQ >= kBlock || rq < KR / 4)
+                    if (W::AQ >= W::T || rq < KR / 4)
                         put(row + s * OCT * BM, rq, pack_exact<DT>(v[0], v[1]), pack_exact<DT>(v[2], v[3]));
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[i] = rest8<odd.value>(v[i]);
@@ -250,10 +260,10 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
                 const unsigned lo = from.g[q].pair(0, j, have), hi = from.g[q].pair(2, j, have);
                 sum[j] = add_pair<DT>(sum[j], lo);
                 sum[CH + j] = add_pair<DT>(sum[CH + j], hi);
-                if (W::AQ >= kBlock || rq < KR / 4) put(row, rq, lo, hi);
+                if (W::AQ >= W::T || rq < KR / 4) put(row, rq, lo, hi);
             }
         } else {
-            const int m = n - CH * NA, q = m >> 2, j = m & 3, rq = br + 8 * q;
+            const int m = n - CH * NA, q = m >> 2, j = m & 3, rq = br + BR * q;
             if (j == 0) {                                         // the word of exponents shifted, and cut to the slice's rows
                 const int r = step * KR + 4 * rq, by = r > last ? r - last : 0;
                 const int have = rows - r < 0 ? 0 : rows - r < 4 ? rows - r : 4;
@@ -269,15 +279,15 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
     };
     // The products of a step out of `from`, and between them, a share behind each PL-th part, whatever `beside` does: matrix cores
     // and vector units work at the same time, from one wave.  Operands are read one part ahead.
-    constexpr int PARTS = KR / 16 * PL;
+    constexpr int PARTS = KR / 16 / GROUPS * PL;
     auto multiply = [&](const u32x4* from, auto beside) {
         u32x4 bf[2][WN], af[2][WM];
         auto read = [&](int part) {
-            const int s = part / PL, k = part % PL;
+            const int sixteen = part / PL, k = part % PL, s = GROUPS * sixteen + group;
             if (k == 0)
 #pragma unroll
                 for (int n = 0; n < WN; ++n)
-                    bf[s & 1][n] = from[PL * OCT * BM + (2 * s + half) * kBN + 32 * (BM == 64 ? 2 * (wid & 1) + n : n) + l31];
+                    bf[sixteen & 1][n] = from[PL * OCT * BM + (2 * s + half) * kBN + 32 * (BM == 64 ? 2 * (wid & 1) + n : n) + l31];
 #pragma unroll
             for (int m = 0; m < WM; ++m)
                 af[part & 1][m] = from[(k * OCT + 2 * s + half) * BM + 32 * (BM == 64 ? wid >> 1 : wid * WM + m) + l31];
@@ -377,38 +387,61 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
         }
     }
 
-    // register r of the lane: tile row (r & 3) + 8 (r >> 2) + 4 half, tile column l31
+    // Two groups: each keeps half of the accumulator registers, 8 g ... 8 g + 7, and takes the other's share of them through LDS.
+    // Register r of the lane: tile row (r & 3) + 8 (r >> 2) + 4 half, tile column l31.
+    float* const swap = reinterpret_cast<float*>(&cells[0][0]);
+    static_assert(GROUPS == 1 || 2 * W::CELLS * 16 >= 8 * WN * 8 * 64 * 4, "the exchange fits into the cells");
 #pragma unroll
     for (int m = 0; m < WM; ++m) {
+        if constexpr (GROUPS == 2) {
+            if (m > 0) __syncthreads();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int at = 32 * (BM == 64 ? wid >> 1 : wid * WM + m) + (r & 3) + 8 * (r >> 2) + 4 * half;
+            for (int n = 0; n < WN; ++n)
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const float low = acc[m][n][r], high = acc[m][n][r + 8];
+                    swap[((wave * WN + n) * 8 + r) * 64 + lane] = group == 0 ? high : low;
+                }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int r = 0; r < 16 / GROUPS; ++r) {
+            const int rr = r + 8 * group;
+            const int at = 32 * (BM == 64 ? wid >> 1 : wid * WM + m) + (rr & 3) + 8 * (rr >> 2) + 4 * half;
             const int o = o0 + W::channel(at), i = i0 + 4 * l31 + (BM == 64 ? 2 * (wid & 1) : 0);
+            float v[WN];
+#pragma unroll
+            for (int n = 0; n < WN; ++n) {
+                if constexpr (GROUPS == 2) {
+                    const float low = acc[m][n][r], high = acc[m][n][(r + 8) & 15];
+                    v[n] = (group == 0 ? low : high) + swap[(((wave ^ 4) * WN + n) * 8 + r) * 64 + lane];
+                } else {
+                    v[n] = acc[m][n][r];
+                }
+            }
             if (o >= p.out) continue;
             if constexpr (WHOLE) {
                 T* const dst = gw + (int64_t)o * p.c + i;
 #pragma unroll
-                for (int n = 0; n < WN; ++n) {
-                    if (i + n < p.c) store_one<DT>(dst + n, alpha * acc[m][n][r]);
-                }
+                for (int n = 0; n < WN; ++n)
+                    if (i + n < p.c) store_one<DT>(dst + n, alpha * v[n]);
             } else if (i < ld) {
                 float* const dst = part + ((int64_t)slice * p.out + o) * ld + i;
-                // (past the caches, written once and read once: 67 -> 64 us on bf16 65536 x 512 x 512)
-                if constexpr (WN == 4)
-                    __builtin_nontemporal_store(f32x4{acc[m][0][r], acc[m][1][r], acc[m][2][r], acc[m][3][r]}, reinterpret_cast<f32x4*>(dst));
-                else
-                    __builtin_nontemporal_store(f32x2{acc[m][0][r], acc[m][1][r]}, reinterpret_cast<f32x2*>(dst));
+                // (past the caches: written once, read once; 67 -> 64 us on bf16 65536 x 512 x 512)
+                if constexpr (WN == 4) __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4*>(dst));
+                else __builtin_nontemporal_store(f32x2{v[0], v[1]}, reinterpret_cast<f32x2*>(dst));
             }
         }
     }
     if (tn == 0 && (WHOLE ? gb != nullptr : part_b != nullptr)) {      // the row quads' sums of each channel, added in order
         constexpr int AG = AR < KR / 4 ? AR : KR / 4;                  // row quads that have one
-        float* const fold = reinterpret_cast<float*>(&cells[0][0]);
+        float* const fold = swap;
+        __syncthreads();
         if (ar < AG)
 #pragma unroll
             for (int j = 0; j < CH; ++j) fold[ar * BM + CH * oq + j] = sum[j] + sum[CH + j];
         __syncthreads();
-        for (int o = tid; o < BM; o += kBlock) {
+        for (int o = tid; o < BM; o += W::T) {
             float t = fold[o];
             for (int rq = 1; rq < AG; ++rq) t += fold[rq * BM + o];
             if (o0 + o >= p.out) continue;
@@ -472,18 +505,16 @@ struct WgPlan {
     WgShape p;
 };
 
-// Tiles of 256 channels of gy and one work-group a CU in f32, whose three pieces fill the matrix cores from one wave a SIMD; of 128 and
-// two work-groups a CU in the 16-bit types, where reading operands takes longer than multiplying them (bf16 65536 x 512 x 512: 63 us
-// so, 68 with the tall tile; f32 16384 x 1024 x 2048: 209 either way).  Shorter ones where those would leave CUs without a work-group
-// of four steps.  Slices so that the work-groups fill the chip once.
+// The tallest tile that leaves no CU without a work-group of four steps (256: one of eight waves a CU; 128, 64: two of four; bf16
+// 65536 x 512 x 512 takes 58 us in tiles of 256, 65 of 128 and 90 of 64).  Slices so that the work-groups fill the chip once.
 WgPlan wg_plan(int64_t rows, int64_t out, int64_t c, int32_t dtype) {
     const int kr = wg_rows(dtype);
     const int64_t steps = ceil_div64(rows, kr), pairs = ceil_div64(steps, 4), tiles_n = ceil_div64(c, kBN);
     int bm = 64;
-    for (int t = dtype == SAE_F32 ? 256 : 128; t > 64; t /= 2)
+    for (int t = 256; t > 64; t /= 2)
         if (out > t / 2 && ceil_div64(out, t) * tiles_n * pairs >= 256) { bm = t; break; }
     const int forced = tuning_knob("SAE_WG_TILE", 0);                       // (tests: every height at small sizes)
-    if (forced && (forced <= 128 || dtype == SAE_F32)) bm = forced;
+    if (forced) bm = forced;
     const int64_t full = bm == 256 ? 256 : 512;
     WgPlan w;
     w.bm = bm;
@@ -522,7 +553,7 @@ template <int DT, int BM, bool ODD>
 void wg_launch(const void* gy, const int8_t* codes, const uint8_t* scales, float* part, float* part_b, void* gw, void* gb, float alpha,
                const WgShape& p, hipStream_t s) {
     using T = typename Elem<DT>::T;
-    const dim3 grid((unsigned)(p.tiles_m * p.tiles_n * p.slices)), block(kBlock);
+    const dim3 grid((unsigned)(p.tiles_m * p.tiles_n * p.slices)), block((unsigned)WgTile<DT, BM>::T);
     if (p.slices == 1)
         hipLaunchKernelGGL((linear_wgrad8_kernel<DT, BM, ODD, true>), grid, block, 0, s, (const T*)gy, codes, scales, part, part_b,
                            (T*)gw, (T*)gb, alpha, p);
@@ -549,7 +580,7 @@ int wg_run(const void* gy, const int8_t* codes, const uint8_t* scales, void* gw,
     else wg_launch<DT, BM, false>(gy, codes, scales, ws, part_b, gw, gb, alpha, p, s)
     if (w.bm == 64) { SAE_WG(64); }
     else if (w.bm == 128) { SAE_WG(128); }
-    else if constexpr (DT == SAE_F32) { SAE_WG(256); }
+    else { SAE_WG(256); }
 #undef SAE_WG
     if (p.slices > 1)
         hipLaunchKernelGGL((linear_wgrad8_reduce_kernel<DT>), dim3((unsigned)ceil_div64(out * p.blocks * kBlk8, 256)),
