@@ -279,8 +279,9 @@ __global__ __launch_bounds__(kWave) void gn_totals_kernel(const double2* __restr
     const int g = blockIdx.x, n = blockIdx.y;
     const int per = p.units / p.groups;
     double a = 0.0, b = 0.0;
-    for (int i = threadIdx.x; i < p.chunks * per; i += kWave) {
-        const int chunk = i / per, u = i - chunk * per;
+    const unsigned records = (unsigned)p.chunks * (unsigned)per;   // (below 2^31)
+    for (unsigned i = threadIdx.x; i < records; i += kWave) {
+        const unsigned chunk = i / (unsigned)per, u = i - chunk * (unsigned)per;
         const double2 t = rec[((int64_t)n * p.chunks + chunk) * p.units + g * per + u];
         a += t.x;
         b += t.y;
@@ -902,7 +903,7 @@ void gn_forward_as(const GnArgs& a, const GnShape& p) {
         hipLaunchKernelGGL((gn_sums_kernel<DT, ANY, true>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
     else
         hipLaunchKernelGGL((gn_sums_kernel<DT, ANY, false>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
-    if (p.groups <= kFoldGroups && p.chunks * p.units <= kFoldRecords) {
+    if (p.groups <= kFoldGroups && (int64_t)p.chunks * p.units <= kFoldRecords) {
         hipLaunchKernelGGL((gn_apply_kernel<DT, ANY, ACT, true>), grid, block, 0, a.stream, (const T*)a.x, (const double2*)rec, a.mean,
                            a.rstd, a.weight, a.bias, (T*)a.out, a.eps, a.slope, a.scale, p);
         return;

@@ -181,7 +181,8 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
     const int64_t r_begin = slice * p.slice_rows;
     const int64_t r_end = r_begin + p.slice_rows < p.rows ? r_begin + p.slice_rows : p.rows;
     const int rows = (int)(r_end - r_begin), steps = (rows + KR - 1) / KR;
-    const int last = (int)(p.rows - r_begin) - 4;
+    const int64_t behind = p.rows - r_begin;                      // (a slice has fewer than 2^26 rows)
+    const int last = (int)(behind < (1 << 30) ? behind : 1 << 30) - 4;
     const int64_t ld = (int64_t)p.blocks * kBlk8;
 
     f32x16 acc[WM][WN];

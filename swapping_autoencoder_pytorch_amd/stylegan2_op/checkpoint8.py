@@ -167,6 +167,8 @@ class _Kept:
 def _pack(t, least):
     if t.dtype not in hip_lib.element_types() or t.numel() < least or _own_or_view_of_leaf(t):
         return t
+    if not t.is_cuda and hip_lib.get().device_only:
+        return t
     order = sorted(range(t.dim()), key=lambda d: (-t.stride(d), d))
     flat = t.detach().permute(order)
     if not flat.is_contiguous():          # expanded, overlapping or with gaps: as it is
@@ -189,7 +191,7 @@ def _unpack(k):
 def activation_checkpoints8(least=65536, enabled=True):
     """Every autograd node built inside keeps the activations it saves (float32, bfloat16, float16; at least ``least`` values) as
     8-bit checkpoints and gets them back when its backward runs, wherever that is.  Leaves that require a gradient (parameters,
-    and what is a view of one) and small tensors are kept as they are.  Forward values do not change; gradients are those at the
+    and what is a view of one), small tensors and host tensors are kept as they are.  Forward values do not change; gradients are those at the
     values that the checkpoints stand for."""
     if not enabled:
         yield

@@ -43,16 +43,17 @@ class GroupNormActFunction(Function):
     def forward(ctx, x, weight, bias, groups, eps, act, slope, scale, keep):
         y, x, stats, codes, scales = _forward(hip_lib.get(), x, weight, bias, groups, eps, act, slope, scale, keep)
         if keep:
-            ctx.save_for_backward(weight, bias, stats, None, codes, scales)
+            ctx.save_for_backward(weight, bias, None, codes, scales)
         else:
-            ctx.save_for_backward(weight, bias, stats, x, None, None)
+            ctx.save_for_backward(weight, bias, x, None, None)
+        ctx.stats = stats                                  # (no activation: saved-tensor hooks that round those leave it alone)
         ctx.cfg = (groups, act, slope, scale)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        weight, bias, stats, x, codes, scales = ctx.saved_tensors
+        weight, bias, x, codes, scales = ctx.saved_tensors
         groups, act, slope, scale = ctx.cfg
         lib = hip_lib.get()
         code = lib.check_channels_last(gy)
@@ -66,7 +67,7 @@ class GroupNormActFunction(Function):
         n_ws = lib.query("group_norm_act_workspace", n, l, c, groups, code, 1)
         ws = gy.new_empty((n_ws,), dtype=torch.uint8) if n_ws else None
         ptr = hip_lib.ptr
-        mean = stats.data_ptr()
+        mean = ctx.stats.data_ptr()
         lib.call_on(gy, "group_norm_act_bwd", gy.data_ptr(), ptr(x), ptr(codes), ptr(scales), mean, mean + 4 * n * groups,
                     ptr(weight), ptr(bias), ptr(gx), ptr(gw), ptr(gb), n, l, c, groups, act, slope, scale, code, ptr(ws), n_ws)
         return gx, gw, gb, None, None, None, None, None, None

@@ -104,6 +104,14 @@ def test_no_cpu_path():
             call()
 
 
+def test_context_leaves_host_tensors():
+    """what the product's library does not take is kept as it is"""
+    x = torch.randn(50, 40, requires_grad=True)
+    with ops.activation_checkpoints8(least=1):
+        y = (x * 1.5) ** 2
+    assert torch.equal(torch.autograd.grad(y.sum(), x)[0], 2 * (x.detach() * 1.5) * 1.5)
+
+
 # ---- values -------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -314,6 +322,15 @@ def check_context(device):
     size = sum(g[i].abs() @ flat[i].abs().t() for i in range(2))
     assert ((gw.cpu().double().view(16, 8) - want).abs() <= 2 * K.E32 * 1200 * size).all()
     assert not torch.equal(gw, plain[2])
+    # a norm's statistics are no activations: its gradients at a leaf are the same inside
+    x8 = K.seeded((4, 16, 6, 5), 6).to(device).contiguous(memory_format=torch.channels_last).requires_grad_()
+    for keep in (False, True):
+        both = []
+        for on in (False, True):
+            with ops.activation_checkpoints8(least=40, enabled=on):
+                y = ops.group_norm_act(x8, 8, b, b, activation="silu", checkpoint=keep)
+            both.append(torch.autograd.grad(y, [x8, b], torch.cos(y.detach())))
+        assert all(torch.equal(a, b) for a, b in zip(*both))
     # channels-last, strided and odd-sized saved tensors come back in their order
     for t in (x.detach().movedim(1, -1), x.detach()[:, :, 1:, 1:], x.detach()[:, :3].contiguous()):
         with ops.activation_checkpoints8(least=64):
@@ -321,6 +338,40 @@ def check_context(device):
             v = (a * 1.0) ** 2
         ga, = torch.autograd.grad(v.sum(), a)
         assert ga.shape == t.shape and ((ga - 2 * t).abs() <= t.abs().max() * 2.0 ** -5).all()
+
+
+def check_parts(device):
+    """each subset of the inputs that can require a gradient gets the same gradients bit for bit; a broadcast gradient, no autograd,
+    3 and 5 dimensions, the module"""
+    for keep in (False, True):
+        for space in ((3, 4), (40, 50)):
+            x = K.seeded((3, 24) + space, 1).to(device).contiguous(memory_format=torch.channels_last)
+            w, b = K.seeded((24,), 2).to(device), K.seeded((24,), 3).to(device)
+            gy = K.seeded((3, 24) + space, 4).to(device)
+
+            def grads(on, gy=gy):
+                leaves = [t.clone().requires_grad_(o) for t, o in zip((x, w, b), on)]
+                y = ops.group_norm_act(leaves[0], 4, *leaves[1:], activation="silu", checkpoint=keep)
+                got = iter(torch.autograd.grad(y, [t for t in leaves if t.requires_grad], gy))
+                return [y.detach()] + [next(got) if o else None for o in on]
+            whole = grads((True, True, True))
+            for on in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (True, False, True)):
+                for got, want in zip(grads(on), whole):
+                    assert got is None or torch.equal(got, want), on
+            one = torch.ones((), device=device)
+            assert all(torch.equal(a, c) for a, c in zip(grads((True,) * 3, one.expand(gy.shape)), grads((True,) * 3, one.expand(gy.shape).clone())))
+            with torch.no_grad():
+                assert torch.equal(ops.group_norm_act(x, 4, w, b, activation="silu", checkpoint=keep), whole[0])
+    flat = ops.group_norm_act(x.flatten(2), 4, w, b)
+    assert torch.equal(flat, ops.group_norm_act(x, 4, w, b).flatten(2))
+    assert torch.equal(ops.group_norm_act(x.unsqueeze(2), 4, w, b), ops.group_norm_act(x, 4, w, b).unsqueeze(2))
+    m, other = ops.GroupNormAct(4, 24, activation="silu").to(device), ops.GroupNormAct(4, 24, activation="silu", checkpoint=True).to(device)
+    with torch.no_grad():
+        m.weight.copy_(w)
+        m.bias.copy_(b)
+    assert sorted(m.state_dict()) == ["bias", "weight"]
+    other.load_state_dict(m.state_dict())
+    assert torch.equal(m(x), other(x)) and torch.equal(m(x), ops.group_norm_act(x, 4, w, b, activation="silu"))
 
 
 @pytest.mark.parametrize("tile", [64, 128, 256])
@@ -333,7 +384,7 @@ def test_wgrad_every_tile_emulated(emu_lib, dtype, tile, monkeypatch):
             K.check_wgrad("cpu", K.TYPES[dtype], shape)
 
 
-CHECKS = [check_memory_orders, check_empty, check_not_finite, check_linear8, check_run_together, check_context]
+CHECKS = [check_memory_orders, check_empty, check_not_finite, check_linear8, check_run_together, check_context, check_parts]
 
 
 @pytest.mark.parametrize("check", CHECKS, ids=lambda f: f.__name__[6:])
@@ -379,6 +430,116 @@ def test_gpu_wgrad_large(dtype, shape):
 @pytest.mark.parametrize("check", CHECKS, ids=lambda f: f.__name__[6:])
 def test_gpu_in_use(check):
     check("cuda:0")
+
+
+def _room(gib):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gib * 2 ** 30:
+        pytest.skip("needs %d GiB of device memory" % gib)
+
+
+@pytest.mark.gpu
+def test_gpu_checkpoint8_past_32_bits():
+    """more than 2^31 values: the rows behind are those of a checkpoint of themselves"""
+    _room(32)
+    x = torch.empty(2 ** 21 + 5, 1030, dtype=torch.bfloat16, device="cuda").normal_()
+    kept = ops.checkpoint8(x)
+    back = kept.dequantize()
+    for part in (slice(0, 9), slice(2 ** 31 // 1056 - 4, 2 ** 31 // 1056 + 4), slice(2 ** 31 // 1030 - 4, 2 ** 31 // 1030 + 4), slice(2 ** 21 - 6, None)):
+        own = ops.checkpoint8(x[part])
+        assert torch.equal(kept.codes[part], own.codes) and torch.equal(kept.scales[:, part], own.scales)
+        assert torch.equal(back[part], own.dequantize())
+
+
+@pytest.mark.gpu
+def test_gpu_norm_past_32_bits():
+    """one sample of more than 2^31 values, kept in 8 bits: positions at both ends against the formulas"""
+    _room(64)
+    l, c, groups = 2 ** 25 + 7, 64, 8
+    x = torch.empty(1, l, c, dtype=torch.bfloat16, device="cuda").normal_(0.5, 1.0).movedim(-1, 1).requires_grad_()
+    gy = torch.empty(1, l, c, dtype=torch.bfloat16, device="cuda").normal_(0.1, 0.1).movedim(-1, 1)
+    w = K.seeded((c,), 1).cuda().requires_grad_()
+    y = ops.group_norm_act(x, groups, w, None, activation="silu", checkpoint=True)
+    gx, gw = torch.autograd.grad(y, [x, w], gy)
+    kept = ops.checkpoint8(x.detach().movedim(1, -1)).dequantize()[0]
+    xs, gs, w64 = x.detach()[0].t(), gy[0].t(), w.detach().double()
+    step = 2 ** 21
+    s1 = sum(xs[i:i + step].double().view(-1, groups, 8).sum((0, 2)) for i in range(0, l, step))
+    mean = (s1 / (8 * l)).repeat_interleave(8)
+    s2 = sum(((xs[i:i + step].double() - mean) ** 2).view(-1, groups, 8).sum((0, 2)) for i in range(0, l, step))
+    rstd = ((s2 / (8 * l)) + 1e-5).rsqrt().repeat_interleave(8)
+
+    def dz_of(part):
+        xh = (kept[part].double() - mean) * rstd
+        s = torch.sigmoid(xh * w64)
+        return gs[part].double() * s * (1 + xh * w64 * (1 - s)), xh
+    sums = torch.zeros(4, c, dtype=torch.float64, device="cuda")              # of w dz, w dz xh, dz xh and |dz xh| + |dz|
+    for i in range(0, l, step):
+        dz, xh = dz_of(slice(i, i + step))
+        sums += torch.stack([(w64 * dz).sum(0), (w64 * dz * xh).sum(0), (dz * xh).sum(0), (dz * xh).abs().sum(0) + dz.abs().sum(0)])
+    m1, m2 = (t.view(groups, 8).sum(1).repeat_interleave(8) / (8 * l) for t in sums[:2])
+    # a thread adds at most 1024 rows; what is in front of the sums is off by 32 roundings of values of at most 1 + |z| at most
+    count, u = 1024, K.half_step(torch.bfloat16)
+    assert ((gw.double() - sums[2]).abs() <= (count + 32 * 8) * K.E32 * sums[3]).all()
+    for part in (slice(0, 500), slice(l - 500, l)):
+        z = (xs[part].double() - mean) * rstd * w64
+        want = z * torch.sigmoid(z)
+        assert ((y.detach()[0].t()[part].double() - want).abs() <= u * want.abs() + 32 * K.E32 * (1 + z.abs()) ** 2).all()
+        dz, xh = dz_of(part)
+        want = rstd * (w64 * dz - m1 - xh * m2)
+        size = rstd * (1 + xh.abs()) * ((w64 * dz).abs() + 1) * (1 + (xh * w64).abs())
+        assert ((gx[0].t()[part].double() - want).abs() <= u * want.abs() + (32 + count) * K.E32 * size).all()
+
+
+@pytest.mark.gpu
+def test_gpu_wgrad_past_32_bits():
+    """more than 2^31 rows, zeros but for both ends and the middle"""
+    _room(96)
+    rows, n = 2 ** 31 + 101, 300
+    gy = torch.zeros(rows, 1, dtype=torch.float16, device="cuda")
+    codes = torch.zeros(rows, 32, dtype=torch.int8, device="cuda")
+    scales = torch.full((1, rows), 127, dtype=torch.uint8, device="cuda")
+    want = torch.zeros(2, 8, dtype=torch.float64, device="cuda")
+    for i, at in enumerate((0, 2 ** 30 + 77, rows - n)):
+        x, g = K.seeded((n, 8), i, torch.float16).cuda(), K.seeded((n, 1), 5 + i, torch.float16).cuda()
+        own = ops.checkpoint8(x)
+        codes[at:at + n], scales[:, at:at + n], gy[at:at + n] = own.codes, own.scales, g
+        v = g.double() * own.dequantize().double()
+        want += torch.stack([v.sum(0), v.abs().sum(0)])
+    gw, gb = ops.linear_weight_grad8(gy, ops.Checkpoint8(codes, scales, 8, torch.float16))
+    u = K.half_step(torch.float16)
+    assert ((gw[0].double() - want[0]).abs() <= 2 * K.E32 * (3 * n + 32) * want[1] * (1 + u) + u * want[0].abs()).all()
+    assert abs(float(gb) - float(gy.double().sum())) <= 2 * K.E32 * (3 * n + 32) * float(gy.abs().double().sum()) * (1 + u) + u * abs(float(gy.double().sum()))
+
+
+@pytest.mark.gpu
+def test_gpu_two_graphs():
+    """two captured steps, replayed in turn and on another stream: each keeps its own workspaces and results"""
+    cases = [_step_inputs(30), _step_inputs(40, torch.bfloat16)]
+    graphs, outs = [], []
+    for c in cases:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _step(*c)
+        torch.cuda.current_stream().wait_stream(side)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(_step(*c))
+    want = [_step(*c) for c in cases]
+    other = torch.cuda.Stream()
+    for turn in range(4):
+        for t in outs[0] + outs[1]:
+            t.detach().zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other if turn % 2 else torch.cuda.current_stream()):
+            graphs[0].replay()
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(got, ref)), turn
+        _step(*cases[turn % 2])                                               # eager work in between
+        torch.cuda.synchronize()
 
 
 def _step(x, w, b, gy, wl, gz):
