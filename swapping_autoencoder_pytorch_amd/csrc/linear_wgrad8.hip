@@ -19,13 +19,16 @@
 // stores, no shuffle.
 //
 // What bounds it: a wave issues in order, so everything a step needs beside its products -- cutting gy, decoding codes, LDS writes,
-// the loads two steps ahead -- is dealt out between them (`multiply`).  Measured (f32 16384 x 1024 x 2048, bf16 65536 x 512 x 512):
+// the loads two and three steps ahead -- is dealt out between them (`multiply`), 6 to 7 vector instructions a product, and two waves a
+// SIMD cover each other.  Measured (f32 16384 x 1024 x 2048, bf16 65536 x 512 x 512, with the reduction):
 //     340, 140 us   one set of cells, a burst of loads, then of vector work, then of products
 //     229, 100      two groups of four waves that stage and multiply in turn; their loads, one step ahead, are waited for
 //     207, 65       four waves, dealt out; operands read ahead
-//     205, 58       eight waves (this form): two on a SIMD to cover each other
-// f32: 1010 - 1040 TFLOP/s on the matrix cores (a library's bf16 product of 8192^3 reaches 1217 on this card; with gy = 0 the same
-// launch takes 177 us: the clock).  bf16: 44 us here and 12 in the kernel that adds the slices; at 65536 x 1024 x 2048 870 TFLOP/s.
+//     201, 58       eight waves, two on a SIMD
+//     192, 58       no branch in a step, no code decoded twice (this form)
+// f32: 1070 TFLOP/s on the matrix cores, where a library's bf16 product of 8192^3 reaches 1217 on this card; the clock is what is left
+// (with gy = 0 the same launch takes 15 % less).  bf16: 45 us here and 12 in the kernel that adds the slices; of the 45, some 10 are
+// the first loads and the last stores.  65536 x 1024 x 2048 runs at 870 TFLOP/s.
 //
 // Few tiles: the rows are cut into slices, one work-group each, whose fp32 tiles a second kernel adds in order.
 #include "elem8.inc"
@@ -150,6 +153,7 @@ struct WgTile {
     static constexpr int BQ = kBN / 4 * (KR / 4);                 // codes quads of a step
     static constexpr int NB = BQ / T > 0 ? BQ / T : 1;            // of a thread
     static constexpr int BR = (T < BQ ? T : BQ) / 32;             // row quads of codes at once
+    static constexpr int BJ = T > BQ ? 2 : 4;                     // codes of a quad that a thread takes of each row
     static constexpr int WM = BM == 256 ? 2 : 1;                  // 32-channel tiles of a wave: 64 x 128 (BM 256),
     static constexpr int WN = BM == 64 ? 2 : 4;                   // 32 x 128 (128), 32 x 64 (64)
     static constexpr int CELLS = OCT * (PL * BM + kBN);           // 16-byte cells of a step
@@ -167,7 +171,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
     using W = WgTile<DT, BM>;
     using T = typename Elem<DT>::T;
     constexpr int PL = W::PL, KR = W::KR, OCT = W::OCT, NA = W::NA, NB = W::NB, WM = W::WM, WN = W::WN, AR = W::AR,
-                  CH = W::CH, BR = W::BR, GROUPS = W::GROUPS;
+                  CH = W::CH, BR = W::BR, BJ = W::BJ, GROUPS = W::GROUPS;
     __shared__ u32x4 cells[2][W::CELLS];                          // of a step: gy [PL][OCT][BM], codes [OCT][kBN]
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wid = wave & 3, group = wave >> 2;
@@ -197,7 +201,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
     Load load[2];
     // neighbouring lanes take the two row quads of a cell: their 8-byte writes fill whole cells, without a bank conflict
     const int oq = (tid >> 1) % (BM / CH), ar = (tid & 1) + 2 * (tid / (2 * BM / CH));   // gy: channels, row quad (of every AR)
-    const int bt = tid % (32 * BR);                              // (more threads than quads: the second half stages the same again)
+    const int bt = tid % (32 * BR), bj = BJ * (tid / (32 * BR));  // (twice as many threads as quads: two codes of each)
     const int bq = (bt >> 1) & 31, br = (bt & 1) + 2 * (bt >> 6);                        // codes: channel quad, row quad (of every BR)
     const bool a_in = W::AQ >= W::T || ar < KR / 4, b_in = i0 + 4 * bq < ld;
     const __amdgpu_buffer_rsrc_t grows = rows_of(gy + r_begin * p.out, ((int64_t)rows * p.out * (int64_t)sizeof(T) + 3) & ~(int64_t)3);
@@ -206,7 +210,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
     const unsigned nowhere = 0xfffffff0u;                         // behind every descriptor
     const unsigned gat = a_in && o0 + CH * oq < p.out
                              ? ((unsigned)(4 * ar) * (unsigned)p.out + (unsigned)(o0 + CH * oq)) * (unsigned)sizeof(T) : nowhere;
-    const unsigned cat = b_in ? (unsigned)(4 * br) * (unsigned)ld + (unsigned)(i0 + 4 * bq) : nowhere;
+    const unsigned cat = b_in ? (unsigned)(4 * br) * (unsigned)ld + (unsigned)(i0 + 4 * bq + bj) : nowhere;
 
     auto fetch_gy = [&](Load& to, int step, int n) {              // n < 4 NA: one row of a box
         to.g[n >> 2].load(n & 3, grows, gat, step * KR + 4 * AR * (n >> 2), rows, p.out);
@@ -215,13 +219,15 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
         const int q = n / 5, i = n % 5;
         if (i < 4) {
             const int from = step * KR + 4 * BR * q + i;
-            to.cw[q][i] = __builtin_amdgcn_raw_buffer_load_b32(crows, cat, (unsigned)(from < rows ? from : rows) * (unsigned)ld, 0);
+            const unsigned at = (unsigned)(from < rows ? from : rows) * (unsigned)ld;
+            if constexpr (BJ == 4) to.cw[q][i] = __builtin_amdgcn_raw_buffer_load_b32(crows, cat, at, 0);
+            else to.cw[q][i] = __builtin_amdgcn_raw_buffer_load_b16(crows, cat, at, 0);
             return;
         }
         const int r = step * KR + 4 * (br + BR * q);
-        if (p.rows >= 4) {                                        // a word that ends at the block's last row at most
+        if (!(BM == 64 && WHOLE) || p.rows >= 4) {                // a word that ends at the block's last row at most
             __builtin_memcpy(&to.ce[q], ssrc + (r < last ? r : last), 4);
-        } else {
+        } else {                                                  // (wg_plan: no other form gets so few rows, nor this branch)
             to.ce[q] = 0;
             for (int i = 0; i < rows; ++i) to.ce[q] |= (unsigned)ssrc[i] << (8 * i);
             to.ce[q] <<= 8 * -last;
@@ -236,7 +242,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
     };
     auto put = [&](u32x4* cell, int rq, unsigned lo, unsigned hi) { *(reinterpret_cast<u32x2*>(cell) + (rq & 1)) = u32x2{lo, hi}; };
     // One channel of a box: of gy (n < CH NA) or of the codes.  odd: with infinities and NaN among the values (f32)
-    constexpr int PIECES = CH * NA + 4 * NB;
+    constexpr int PIECES = CH * NA + BJ * NB;
     auto stage = [&](const Load& from, int step, u32x4* to, int n, auto odd) {
         if (n < CH * NA) {
             const int q = n / CH, j = n % CH, rq = ar + AR * q;
@@ -264,7 +270,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
                 if (W::AQ >= W::T || rq < KR / 4) put(row, rq, lo, hi);
             }
         } else {
-            const int m = n - CH * NA, q = m >> 2, j = m & 3, rq = br + BR * q;
+            const int m = n - CH * NA, q = m / BJ, j = m % BJ, rq = br + BR * q;
             if (j == 0) {                                         // the word of exponents shifted, and cut to the slice's rows
                 const int r = step * KR + 4 * rq, by = r > last ? r - last : 0;
                 const int have = rows - r < 0 ? 0 : rows - r < 4 ? rows - r : 4;
@@ -275,11 +281,11 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
             float v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(from.cw[q][i] >> (8 * j)) * pace[q][i];
-            put(to + PL * OCT * BM + (rq >> 1) * kBN + 32 * j + bq, rq, pack_exact<DT>(v[0], v[1]), pack_exact<DT>(v[2], v[3]));
+            put(to + PL * OCT * BM + (rq >> 1) * kBN + 32 * (bj + j) + bq, rq, pack_exact<DT>(v[0], v[1]), pack_exact<DT>(v[2], v[3]));
         }
     };
     // The products of a step out of `from`, and between them, a share behind each PL-th part, whatever `beside` does: matrix cores
-    // and vector units work at the same time, from one wave.  Operands are read one part ahead.
+    // and vector units work at the same time.  Operands are read one part ahead.
     constexpr int PARTS = KR / 16 / GROUPS * PL;
     auto multiply = [&](const u32x4* from, auto beside) {
         u32x4 bf[2][WN], af[2][WM];
@@ -308,7 +314,7 @@ void linear_wgrad8_kernel(const typename Elem<DT>::T* __restrict__ gy, const int
 #pragma unroll
             for (int i = 0; i < WM * WN; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, DT == SAE_F32 ? 6 : 9, 0);    // (the other way round: 1 % more each)
                 __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
             }
@@ -511,11 +517,11 @@ struct WgPlan {
 WgPlan wg_plan(int64_t rows, int64_t out, int64_t c, int32_t dtype) {
     const int kr = wg_rows(dtype);
     const int64_t steps = ceil_div64(rows, kr), pairs = ceil_div64(steps, 4), tiles_n = ceil_div64(c, kBN);
-    int bm = 64;
-    for (int t = 256; t > 64; t /= 2)
+    int bm = 64;                                                            // (fewer than four rows: the form that reads so few)
+    for (int t = 256; t > 64 && rows >= 4; t /= 2)
         if (out > t / 2 && ceil_div64(out, t) * tiles_n * pairs >= 256) { bm = t; break; }
     const int forced = tuning_knob("SAE_WG_TILE", 0);                       // (tests: every height at small sizes)
-    if (forced) bm = forced;
+    if (forced && rows >= 4) bm = forced;
     const int64_t full = bm == 256 ? 256 : 512;
     WgPlan w;
     w.bm = bm;

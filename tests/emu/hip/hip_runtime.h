@@ -422,12 +422,22 @@ inline unsigned raw_buffer_load1(hipemu_rsrc r, unsigned voffset, unsigned soffs
     }
     return v;
 }
+inline unsigned short raw_buffer_load_half(hipemu_rsrc r, unsigned voffset, unsigned soffset) {
+    unsigned short v = 0;
+    if ((unsigned long long)voffset + soffset + 2 <= r.num_records) {
+        const char* a = r.base + soffset + voffset;
+        if (a + 2 > hipemu_guard_lo && a < hipemu_guard_hi) ++hipemu_guard_count;
+        else std::memcpy(&v, a, 2);
+    }
+    return v;
+}
 }  // namespace hipemu
 #define __amdgpu_buffer_rsrc_t hipemu_rsrc
 #define __builtin_amdgcn_make_buffer_rsrc(p, stride, num, flags) (hipemu_rsrc{(const char*)(p), (unsigned)(num)})
 #define __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, aux) hipemu::raw_buffer_load<hipemu_u32x4, 4>((r), (unsigned)(voff), (unsigned)(soff))
 #define __builtin_amdgcn_raw_buffer_load_b64(r, voff, soff, aux) hipemu::raw_buffer_load<hipemu_u32x2, 2>((r), (unsigned)(voff), (unsigned)(soff))
 #define __builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, aux) hipemu::raw_buffer_load1((r), (unsigned)(voff), (unsigned)(soff))
+#define __builtin_amdgcn_raw_buffer_load_b16(r, voff, soff, aux) hipemu::raw_buffer_load_half((r), (unsigned)(voff), (unsigned)(soff))
 
 template <typename T>
 static inline T __shfl_xor(T v, int mask, int width = 64) {

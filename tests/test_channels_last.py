@@ -380,7 +380,7 @@ def test_wgrad_every_tile_emulated(emu_lib, dtype, tile, monkeypatch):
     """the tile heights that small sizes do not reach by themselves (the knob exists in tuning builds only)"""
     monkeypatch.setenv("SAE_WG_TILE", str(tile))
     with backend(emu_lib):
-        for shape in ((70, 130, 300), (33, 40, 7), (300, 64, 129)):
+        for shape in ((70, 130, 300), (33, 40, 7), (300, 64, 129), (3, 40, 70), (4, 33, 65)):
             K.check_wgrad("cpu", K.TYPES[dtype], shape)
 
 
@@ -419,7 +419,7 @@ def test_gpu_wgrad(dtype, shape):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [(2000, 640, 1100), (4100, 1030, 2048), (1025, 2048, 513), (20000, 256, 250)], ids=lambda s: "r%d_c%d_o%d" % s)
+@pytest.mark.parametrize("shape", [(2000, 640, 1100), (4100, 1030, 2048), (1025, 2048, 513), (20000, 256, 250), (3, 2048, 16384), (4, 2048, 16384)], ids=lambda s: "r%d_c%d_o%d" % s)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gpu_wgrad_large(dtype, shape):
     """sizes that fill the chip: the tall tiles, slices for every XCD"""
