@@ -16,6 +16,12 @@
 // Layout of a walk: a lane owns V neighbouring channels (16 bytes) and takes four rows at a time, so that four loads are under way
 // and the exponents of four rows are one word.  ANY: rows (or slabs of them) that start anywhere and end inside a vector.
 //
+// What bounds it: HBM, each tensor's bytes twice less what the caches keep.  f32 [16, 128, 256, 256] kept in 8 bits (537 MB): sums 131 us
+// (678 MB, 5.2 TB/s), apply 201 (1074 MB, 5.3), backward sums 120 (678 MB, 5.6), apply 212 (1213 MB, 5.7).  f32 [16, 512, 64, 64]
+// (134 MB): 26 + 5 + 42 us, 43 + 6 + 61 back, 212 in all a row at a time, stores through the caches, first chunk first.  bf16
+// [16, 256, 64, 64] forward: 9.3 + 14.5 us (36 so).  In groups of samples that the 256 MB cache would hold the
+// largest takes 2 - 50 % longer (more kernels' ends).
+//
 // Numerics: a thread adds x - x0 and (x - x0)^2 over its rows, x0 the first value it meets in the channel: at most the number of
 // its rows times the rounding of a plain sum, whatever the channel's mean.  The records are moments about zero in 64 bits, which
 // only have to be added.  mean and rstd are fp32; nothing is held in less.
@@ -818,7 +824,7 @@ int gn_slab(int64_t c, int64_t groups, int v, int esize, GnCodes codes) {
     return 0;
 }
 
-GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int esize, GnCodes codes) {
+GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int esize, GnCodes codes, bool backward) {
     const int v = 16 / esize;
     GnShape p;
     p.l = l;
@@ -830,11 +836,15 @@ GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int esize, GnCo
     p.units = p.cg % v == 0 ? (int)c / v : (int)c;
     p.slab = gn_slab(c, groups, v, esize, codes);
     p.slabs = p.slab ? (int)ceil_div64(groups, p.slab) : 0;
-    // One launch where a thread of kFused makes at most 8 / kQ trips over its slab, twice; 16 where the whole tensor is so small (4 MB)
-    // that launches are what costs.  (knob 0, for tests: never)
+    // One launch where a thread of kFused has at most 64 values of its slab (backward: 32) and the tensor is small.  Against three
+    // (two) launches, n of 1 ... 64, c of 96 ... 512, f32 and bf16:    forward, <= 10 MB: 16 values -30 ... -47 %, 40 -10 ... -38 %,
+    // 64 -37 ... +4 %, 128 (bf16) +22 ... +43 %; 12 to 18 MB -11 ... +21 %, 32 MB +17 ... +26 %.    backward, <= 4 MB: 8 or 16 values
+    // -43 ... -5 %, 20 -22 ... +3 %, 32 -11 ... +10 % (and a launch or two fewer), 40 -6 ... +17 %; 8 MB -8 ... +10 %, 16 MB +16 %.
+    // (knob 0, for tests: never)
     if (p.slab) {
-        const int64_t trips = ceil_div64(l * p.slab * p.cg, (int64_t)kFused * v) * tuning_knob("SAE_GN_ONE_LAUNCH", 1);
-        if (trips == 0 || trips > (n * l * c * esize <= ((int64_t)4 << 20) ? 16 : 8)) p.slab = 0;
+        const int64_t values = l * p.slab * p.cg, bytes = n * l * c * esize;
+        const bool small = backward ? values <= kFused * 32 && bytes <= ((int64_t)4 << 20) : values <= kFused * 64 && bytes <= ((int64_t)10 << 20);
+        if (!small || tuning_knob("SAE_GN_ONE_LAUNCH", 1) == 0) p.slab = 0;
     }
     // lanes of so many channels; a walk that writes codes has all lanes of a block
     auto lanes_of = [&](int64_t w) { return (int)(codes == kWriteCodes ? ceil_div64(w, kBlk8) * (kBlk8 / v) : ceil_div64(w, v)); };
@@ -969,7 +979,7 @@ void gn_run(const GnArgs& a, const GnShape& p, bool backward) {
 
 int gn_dispatch(const char* what, GnArgs& a, int64_t l, int64_t c, int64_t groups, int32_t dtype, int64_t ws_bytes, bool backward) {
     const GnCodes codes = !a.codes ? kNoCodes : backward ? kReadCodes : kWriteCodes;
-    const GnShape p = gn_plan(a.n, l, c, groups, elem_bytes(dtype), codes);
+    const GnShape p = gn_plan(a.n, l, c, groups, elem_bytes(dtype), codes, backward);
     const int64_t need = gn_workspace(p, a.n, backward);
     if (need > 0 && (!a.ws || ws_bytes < need))
         return fail(SAE_EWORKSPACE, "%s: workspace %lld < %lld bytes (sae_group_norm_act_workspace)", what, (long long)ws_bytes,
@@ -989,8 +999,9 @@ using namespace sae;
 
 extern "C" int64_t sae_group_norm_act_workspace(int64_t n, int64_t l, int64_t c, int64_t groups, int32_t dtype, int32_t backward) {
     if (!gn_shape_ok(n, l, c, groups) || !elem_known(dtype) || n == 0 || l == 0) return 0;
-    const int64_t without = gn_workspace(gn_plan(n, l, c, groups, elem_bytes(dtype), kNoCodes), n, backward != 0);
-    const int64_t with = gn_workspace(gn_plan(n, l, c, groups, elem_bytes(dtype), backward ? kReadCodes : kWriteCodes), n, backward != 0);
+    const int64_t without = gn_workspace(gn_plan(n, l, c, groups, elem_bytes(dtype), kNoCodes, backward != 0), n, backward != 0);
+    const int64_t with = gn_workspace(gn_plan(n, l, c, groups, elem_bytes(dtype), backward ? kReadCodes : kWriteCodes, backward != 0), n,
+                                       backward != 0);
     return with > without ? with : without;
 }
 

@@ -29,10 +29,10 @@
 namespace sae {
 namespace {
 
-// The input transform works on packed pairs -- v_pk_add_f32 with op_sel / neg modifiers (sae_common.h: pk_sub / pk_c01 / pk_c23), 56
-// instead of 84 vector-ALU instructions per thread and chunk -- with V kept in LDS as pairs of POINTS and the MFMA loop walking the
-// points two at a time (+1.3 % on the 128 / 256-channel layers; the scalar form and the packed form of the weight gradient's x
-// side, which measured 4 - 7 % SLOWER, are recorded in profiles/r5_ab_wino_fused_pk.txt and tools/archive/variants/).
+// The input transform works on pairs (sae_common.h: pk_sub / pk_c01 / pk_c23) with V kept in LDS as pairs of POINTS and the MFMA loop
+// walking the points two at a time (the other layouts measured, and the weight gradient's x side in pairs, 4 - 7 % slower, are recorded
+// in profiles/r5_ab_wino_fused_pk.txt and tools/archive/variants/; those figures are of packed instructions, which the library no
+// longer uses).
 
 constexpr int kWfM = 64;       // output channels per workgroup
 constexpr int kWfT = 64;       // 2x2 output tiles per workgroup
