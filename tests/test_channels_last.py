@@ -374,6 +374,23 @@ def check_parts(device):
     assert torch.equal(m(x), other(x)) and torch.equal(m(x), ops.group_norm_act(x, 4, w, b, activation="silu"))
 
 
+def check_context_twice_differentiated(device):
+    """a gradient penalty inside the context: what is saved twice is unpacked with its place in the graph.  Each of the two tensors
+    that are kept here is off by 2^-7 of a block's largest value, at most sqrt(32) of the block's root mean square: 2^-3 together"""
+    x = K.seeded((2, 8, 16, 16), 1).to(device).requires_grad_()
+    w = torch.nn.Parameter(K.seeded((16, 8, 3, 3), 2).to(device))
+    b = torch.nn.Parameter(K.seeded((16,), 3).to(device))
+    got = []
+    for on in (False, True):
+        with ops.activation_checkpoints8(least=64, enabled=on):
+            y = ops.fused_leaky_relu(ops.conv2d(x, w, padding=1), b)
+            g, = torch.autograd.grad((y * torch.cos(y.detach())).sum(), x, create_graph=True)
+            penalty = (g * g).sum()
+        got.append(torch.autograd.grad(penalty, w)[0].double())
+    off = (got[1] - got[0]).norm() / got[0].norm()
+    assert 0 < off <= 2 ** -3
+
+
 @pytest.mark.parametrize("tile", [64, 128, 256])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_wgrad_every_tile_emulated(emu_lib, dtype, tile, monkeypatch):
@@ -384,7 +401,7 @@ def test_wgrad_every_tile_emulated(emu_lib, dtype, tile, monkeypatch):
             K.check_wgrad("cpu", K.TYPES[dtype], shape)
 
 
-CHECKS = [check_memory_orders, check_empty, check_not_finite, check_linear8, check_run_together, check_context, check_parts]
+CHECKS = [check_memory_orders, check_empty, check_not_finite, check_linear8, check_run_together, check_context, check_parts, check_context_twice_differentiated]
 
 
 @pytest.mark.parametrize("check", CHECKS, ids=lambda f: f.__name__[6:])
@@ -510,6 +527,35 @@ def test_gpu_wgrad_past_32_bits():
     u = K.half_step(torch.float16)
     assert ((gw[0].double() - want[0]).abs() <= 2 * K.E32 * (3 * n + 32) * want[1] * (1 + u) + u * want[0].abs()).all()
     assert abs(float(gb) - float(gy.double().sum())) <= 2 * K.E32 * (3 * n + 32) * float(gy.abs().double().sum()) * (1 + u) + u * abs(float(gy.double().sum()))
+
+
+@pytest.mark.gpu
+def test_gpu_context_captured():
+    """the context inside a captured step: replays with new inputs against the eager step"""
+    norm = ops.GroupNormAct(4, 32, activation="silu").cuda()
+    w = torch.nn.Parameter(K.seeded((24, 32), 1).cuda())
+
+    def step(x):
+        with ops.activation_checkpoints8(least=256):
+            y = norm(x * 1.5)
+            z = ops.linear8(y.movedim(1, -1), w)
+        return torch.autograd.grad(z, [norm.weight, norm.bias, w], 2 * z.detach())
+    make = lambda seed: K.seeded((2, 32, 9, 7), seed).cuda().contiguous(memory_format=torch.channels_last)
+    x = make(5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x)
+    for seed in (6, 7, 8):
+        x.copy_(make(seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step(make(seed)))), seed
 
 
 @pytest.mark.gpu
