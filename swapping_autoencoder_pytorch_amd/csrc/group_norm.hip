@@ -9,7 +9,7 @@
 //
 // Every statistic needs the whole group before the first result can be written, so each direction walks its tensors twice:
 //     sums      per (sample, chunk of rows, channel), in registers, one record per chunk
-//     totals    the chunks' records added in order: mean / rstd, or m1 / m2 and the channel sums
+//     totals    the chunks' records added in order: mean / rstd, or m1 / m2 and the channel sums (few records: by the apply kernel)
 //     apply     the elementwise pass, last chunk first: what the sums read last is what the caches still hold
 // or, where a sample's groups are small, all of it in one work-group per (sample, slab of whole groups): one launch.
 //
@@ -301,8 +301,20 @@ __global__ __launch_bounds__(kWave) void gn_totals_kernel(const double2* __restr
     }
 }
 
-// TOTALS: the statistics too, from the sample's records -- each work-group for itself, where they are few
-constexpr int kFoldGroups = 256, kFoldRecords = 1024;
+// Totals by the apply kernels: each work-group adds its sample's records for itself, where they are few (fold_totals); a launch fewer.
+// `per` lanes of a wave, a power of two, for each group; every work-group adds in the same order.
+constexpr int kFoldGroups = kBlock, kFoldChannels = 512;
+__device__ __forceinline__ int fold_lanes(int groups) {
+    int per = kWave;
+    while (per * groups > kBlock) per >>= 1;
+    return per;
+}
+__device__ __forceinline__ double lanes_sum_d(double v, int per) {
+    for (int off = per >> 1; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+
+// TOTALS: the statistics too
 template <int DT, bool ANY, int ACT, bool TOTALS>
 __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const typename Elem<DT>::T* __restrict__ x, const double2* __restrict__ rec,
                                                           float* __restrict__ mean, float* __restrict__ rstd,
@@ -319,29 +331,21 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(const typename Elem<DT
     w.first = (int64_t)chunk * p.chunk_rows;
     w.r_end = w.first + p.chunk_rows < p.l ? w.first + p.chunk_rows : p.l;
     __shared__ float2 stat[TOTALS ? kFoldGroups : 1];
-    __shared__ double2 share[TOTALS ? kBlock : 1];
     if constexpr (TOTALS) {
-        // `per` threads a group (a power of two) take its records in turn, then one adds their shares: the same order in every group
-        const int units = p.units / p.groups, items = p.chunks * units;
-        int per = kBlock;
-        while (per * p.groups > kBlock) per >>= 1;
-        const int g = tid / per, k = tid - g * per;
-        double2 t{0.0, 0.0};
+        const int units = p.units / p.groups, items = p.chunks * units, per = fold_lanes(p.groups), g = tid / per;
+        double a = 0.0, b = 0.0;
         if (g < p.groups)
-            for (int i = k; i < items; i += per) {
+#pragma unroll 4
+            for (int i = tid - g * per; i < items; i += per) {
                 const int at = i / units, u = i - at * units;
                 const double2 o = rec[((int64_t)n * p.chunks + at) * p.units + g * units + u];
-                t.x += o.x;
-                t.y += o.y;
+                a += o.x;
+                b += o.y;
             }
-        share[tid] = t;
-        __syncthreads();
-        if (g < p.groups && k == 0) {
-            for (int i = 1; i < per; ++i) {
-                t.x += share[tid + i].x;
-                t.y += share[tid + i].y;
-            }
-            const float2 s = moments(t.x, t.y, (double)p.l * p.cg, eps);
+        a = lanes_sum_d(a, per);
+        b = lanes_sum_d(b, per);
+        if (g < p.groups && tid == g * per) {
+            const float2 s = moments(a, b, (double)p.l * p.cg, eps);
             stat[g] = s;
             if (chunk == 0) {
                 mean[(int64_t)n * p.groups + g] = s.x;
@@ -689,17 +693,71 @@ __device__ __forceinline__ void bwd_factors(float rs, float2 m, float w, float s
     ge = -rs * m.x;
 }
 
-template <int DT, bool ANY, int ACT, bool KEPT>
+// TOTALS: the two means and the weights' gradients too, from the records of the sums
+template <int DT, bool ANY, int ACT, bool KEPT, bool TOTALS>
 __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const typename Elem<DT>::T* __restrict__ gy,
                                                               const typename Elem<DT>::T* __restrict__ x,
                                                               const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                              const BwdIn in, const float2* __restrict__ means,
+                                                              const BwdIn in, const float2* __restrict__ rec,
+                                                              const float2* __restrict__ means,
                                                               const float2* __restrict__ totals, float* __restrict__ gw,
                                                               float* __restrict__ gb, typename Elem<DT>::T* __restrict__ gx, float slope,
                                                               float scale, const GnShape p) {
     constexpr int V = Elem<DT>::kVec;
     const int n = (int)gridDim.y - 1 - (int)blockIdx.y, chunk = (int)gridDim.x - 1 - (int)blockIdx.x, tid = threadIdx.x;
-    if (totals) {                                                  // gw and gb on the way, 256 channels a work-group
+    __shared__ double2 red[TOTALS ? kBlock : 1];
+    __shared__ double2 sums[TOTALS ? kFoldChannels : 1];
+    __shared__ float2 stat[TOTALS ? kFoldGroups : 1];
+    if constexpr (TOTALS) {
+        const int lane = tid & (kWave - 1), waves = (int)(gridDim.x * gridDim.y) * (kBlock / kWave);
+        if (gw || gb)                                              // a wave a channel, over all samples
+            for (int ch = (int)(blockIdx.y * gridDim.x + blockIdx.x) * (kBlock / kWave) + (tid >> 6); ch < p.c; ch += waves) {
+                double a = 0.0, b = 0.0;
+                for (int i = lane; i < p.chunks * (int)gridDim.y; i += kWave) {
+                    const float2 t = rec[(int64_t)i * p.c + ch];
+                    a += t.x;
+                    b += (double)t.y * in.rstd[(int64_t)(i / p.chunks) * p.groups + ch / p.cg];
+                }
+                a = wave_sum_d(a) * scale;
+                b = wave_sum_d(b) * scale;
+                if (lane == 0 && gb) gb[ch] = (float)a;
+                if (lane == 0 && gw) gw[ch] = (float)b;
+            }
+        if (!gx) return;
+        const int width = p.c < kBlock ? p.c : kBlock, depth = kBlock / width, tx = tid % width, ty = tid / width;
+        for (int u0 = 0; u0 < p.c; u0 += width) {                  // the sample's channels
+            const int ch = u0 + tx;
+            double2 t{0.0, 0.0};
+            if (ch < p.c && ty < depth)
+#pragma unroll 4
+                for (int i = ty; i < p.chunks; i += depth) {
+                    const float2 o = rec[((int64_t)n * p.chunks + i) * p.c + ch];
+                    t.x += o.x;
+                    t.y += o.y;
+                }
+            __syncthreads();
+            red[tid] = t;
+            fold_rows(red, tx, ty, width, depth, ty < depth);
+            if (ty == 0 && ch < p.c) sums[ch] = red[tx];
+        }
+        __syncthreads();
+        const int per = fold_lanes(p.groups), g = tid / per;
+        double m1 = 0.0, m2 = 0.0;
+        if (g < p.groups)
+            for (int u = tid - g * per; u < p.cg; u += per) {
+                const int ch = g * p.cg + u;
+                const double weight = in.weight ? in.weight[ch] : 1.0;
+                m1 += weight * sums[ch].x;
+                m2 += weight * sums[ch].y;
+            }
+        m1 = lanes_sum_d(m1, per);
+        m2 = lanes_sum_d(m2, per);
+        if (g < p.groups && tid == g * per) {
+            const double m = (double)scale / ((double)p.l * p.cg);
+            stat[g] = float2{(float)(m1 * m), (float)(m2 * m * in.rstd[(int64_t)n * p.groups + g])};
+        }
+        __syncthreads();
+    } else if (totals) {                                           // gw and gb on the way, 256 channels a work-group
         const int blocks = (int)(gridDim.x * gridDim.y);
         for (int ch = (int)(blockIdx.y * gridDim.x + blockIdx.x) * kBlock + tid; ch < p.c; ch += blocks * kBlock)
             weight_grads(totals, gw, gb, (int)gridDim.y, p.c, ch);
@@ -728,7 +786,8 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_apply_kernel(const typename Ele
         for (int j = 0; j < V; ++j) {
             if (j == 0 || g[j] != g[j - 1]) {
                 rs = in.rstd[(int64_t)n * p.groups + g[j]];
-                m = means[(int64_t)n * p.groups + g[j]];
+                if constexpr (TOTALS) m = stat[g[j]];
+                else m = means[(int64_t)n * p.groups + g[j]];
             }
             bwd_factors<V>(rs, m, ga[j], scale, ga[j], gd[j], ge[j]);
         }
@@ -894,6 +953,15 @@ struct GnArgs {
     hipStream_t stream;
 };
 
+// The apply kernel adds a sample's records (`bytes` of them) itself: up to 64 KB for each work-group and 32 MB for all.  The GPU takes as
+// long either way (f16 [3, 100, 33, 65] 17.8 + 19.4 against 18.2 + 19.5 us; bf16 [2, 64, 128, 128] in one group 12.3 + 22.2 against
+// 10.9 + 16.9; at 128 KB f16 [8, 320, 1000] 18.5 against 26.2 back), a training step of two launches fewer 4 % less (139 against 133 us).
+// (knob 0, for tests: never)
+bool fold_totals(const GnShape& p, int64_t n, int64_t bytes) {
+    return p.groups <= kFoldGroups && bytes <= ((int64_t)64 << 10) && bytes * p.chunks * n <= ((int64_t)32 << 20) &&
+           tuning_knob("SAE_GN_FOLD", 1) != 0;
+}
+
 template <int DT, bool ANY, int ACT>
 void gn_forward_as(const GnArgs& a, const GnShape& p) {
     using T = typename Elem<DT>::T;
@@ -913,7 +981,7 @@ void gn_forward_as(const GnArgs& a, const GnShape& p) {
         hipLaunchKernelGGL((gn_sums_kernel<DT, ANY, true>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
     else
         hipLaunchKernelGGL((gn_sums_kernel<DT, ANY, false>), grid, block, 0, a.stream, (const T*)a.x, rec, a.codes, a.scales, p);
-    if (p.groups <= kFoldGroups && (int64_t)p.chunks * p.units <= kFoldRecords) {
+    if (fold_totals(p, a.n, (int64_t)p.chunks * p.units * (int64_t)sizeof(double2))) {
         hipLaunchKernelGGL((gn_apply_kernel<DT, ANY, ACT, true>), grid, block, 0, a.stream, (const T*)a.x, (const double2*)rec, a.mean,
                            a.rstd, a.weight, a.bias, (T*)a.out, a.eps, a.slope, a.scale, p);
         return;
@@ -946,11 +1014,17 @@ void gn_backward_as(const GnArgs& a, const GnShape& p) {
     float2* means = totals + a.n * p.c;
     hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, ANY, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
                        (const int8_t*)a.codes, (const uint8_t*)a.scales, in, rec, a.slope, p);
+    if (p.c <= kFoldChannels && fold_totals(p, a.n, (int64_t)p.chunks * p.c * (int64_t)sizeof(float2))) {
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, ANY, ACT, KEPT, true>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
+                           (const int8_t*)a.codes, (const uint8_t*)a.scales, in, (const float2*)rec, (const float2*)nullptr,
+                           (const float2*)nullptr, a.gw, a.gb, (T*)a.out, a.slope, a.scale, p);
+        return;
+    }
     hipLaunchKernelGGL(gn_bwd_totals_kernel, dim3((unsigned)p.groups, (unsigned)a.n), block, 0, a.stream, (const float2*)rec,
                        a.weight, (const float*)a.rstd, totals, means, a.scale, p);
     if (a.out)
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, ANY, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
-                           (const int8_t*)a.codes, (const uint8_t*)a.scales, in, (const float2*)means,
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, ANY, ACT, KEPT, false>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
+                           (const int8_t*)a.codes, (const uint8_t*)a.scales, in, (const float2*)nullptr, (const float2*)means,
                            weights ? (const float2*)totals : (const float2*)nullptr, a.gw, a.gb, (T*)a.out, a.slope, a.scale, p);
     else
         hipLaunchKernelGGL(gn_bwd_weight_kernel, dim3((unsigned)ceil_div(p.c, kBlock)), block, 0, a.stream, (const float2*)totals,

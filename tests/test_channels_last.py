@@ -181,8 +181,11 @@ def test_norm_in_three_launches_emulated(emu_lib, dtype, shape, monkeypatch):
     """small groups through the kernels of the large ones (the knob exists in tuning builds only)"""
     monkeypatch.setenv("SAE_GN_ONE_LAUNCH", "0")
     with backend(emu_lib):
-        K.check_norm("cpu", K.TYPES[dtype], shape, "silu", checkpoint=False)
-        K.check_norm("cpu", K.TYPES[dtype], shape, "lrelu", checkpoint=True)
+        for fold in ("1", "0"):                      # two launches, and with one for the totals
+            monkeypatch.setenv("SAE_GN_FOLD", fold)
+            K.check_norm("cpu", K.TYPES[dtype], shape, "silu", checkpoint=False)
+            K.check_norm("cpu", K.TYPES[dtype], shape, "lrelu", checkpoint=True)
+            K.check_norm("cpu", K.TYPES[dtype], shape, "none", checkpoint=False, affine=False)
 
 
 @pytest.mark.parametrize("shape", K.WGRAD_SHAPES, ids=lambda s: "r%d_c%d_o%d" % s)
