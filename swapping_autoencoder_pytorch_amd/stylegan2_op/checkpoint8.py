@@ -154,9 +154,11 @@ def linear8(input, weight, bias=None, alpha=1.0):
     return Linear8.apply(x2, weight, bias, alpha, train).view(*lead, weight.shape[0])
 
 
-def _own_or_view_of_leaf(t):
+def _lives_anyway(t):
+    """A parameter, trainable or frozen, another leaf that requires a gradient, or a view of one: its memory is not the graph's to
+    free, and a data gradient through it would be taken at rounded weights."""
     base = t if t._base is None else t._base
-    return base.is_leaf and base.requires_grad
+    return isinstance(base, torch.nn.Parameter) or (base.is_leaf and base.requires_grad)
 
 
 class _Kept:
@@ -165,7 +167,7 @@ class _Kept:
 
 
 def _pack(t, least):
-    if t.dtype not in hip_lib.element_types() or t.numel() < least or _own_or_view_of_leaf(t):
+    if t.dtype not in hip_lib.element_types() or t.numel() < least or _lives_anyway(t):
         return t
     if not t.is_cuda and hip_lib.get().device_only:
         return t
@@ -190,9 +192,10 @@ def _unpack(k):
 @contextlib.contextmanager
 def activation_checkpoints8(least=65536, enabled=True):
     """Every autograd node built inside keeps the activations it saves (float32, bfloat16, float16; at least ``least`` values) as
-    8-bit checkpoints and gets them back when its backward runs, wherever that is.  Leaves that require a gradient (parameters,
-    and what is a view of one), small tensors and host tensors are kept as they are.  Forward values do not change; gradients are those at the
-    values that the checkpoints stand for."""
+    8-bit checkpoints and gets them back when its backward runs, wherever that is.  Parameters (trainable or frozen), other leaves
+    that require a gradient, views of either, small tensors and host tensors are kept as they are.  A weight that is no Parameter --
+    detached, or computed from one -- is an activation here.  Forward values do not change; gradients are those at the values that
+    the checkpoints stand for."""
     if not enabled:
         yield
         return

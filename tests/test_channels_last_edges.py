@@ -1,0 +1,57 @@
+"""The channels-last operators at their edges: frozen weights, shared and foreign tensors inside activation_checkpoints8, forward-mode
+differentiation, small gradients, the sizes on both sides of every choice between kernels."""
+import pytest
+import torch
+
+import channels_last_cases as K
+from parity_common import backend
+from swapping_autoencoder_pytorch_amd import hip_lib
+from swapping_autoencoder_pytorch_amd import stylegan2_layers as layers
+from swapping_autoencoder_pytorch_amd import stylegan2_op as ops
+
+
+def _layers(device):
+    """(name, layer of at least 4096 weights, input's shape) of the framework's own layers and operators"""
+    torch.manual_seed(7)
+    conv, matrix = (torch.nn.Parameter(torch.randn(s).to(device)) for s in ((64, 16, 3, 3), (64, 144)))
+    made = [("conv2d", lambda x: ops.conv2d(x, conv, padding=1), [conv], (2, 16, 9, 9)),
+            ("linear", lambda x: ops.linear(x, matrix), [matrix], (5, 144)),
+            ("linear of a view", lambda x: ops.linear(x, conv.view(64, 144)), [conv], (5, 144))]
+    for name, layer, shape in (("EqualLinear", layers.EqualLinear(96, 64, activation="fused_lrelu"), (5, 96)),
+                               ("EqualConv2d", layers.EqualConv2d(32, 32, 3, padding=1), (2, 32, 8, 8)),
+                               ("ConvLayer", layers.ConvLayer(32, 32, 3), (2, 32, 8, 8)),
+                               ("ResBlock", layers.ResBlock(32, 32), (2, 32, 16, 16))):
+        layer = layer.to(device)
+        made.append((name, layer, list(layer.parameters()), shape))
+    return made
+
+
+def check_frozen_parameters(device):
+    """a Parameter is kept as it is whether it requires a gradient or not: the input gradient through a frozen layer is the plain one
+    bit for bit (what is packed besides are the layer's own activations, read by their signs alone)"""
+    for name, layer, params, shape in _layers(device):
+        x = K.seeded(shape, 3).to(device)
+        for p in params:
+            p.requires_grad_(False)
+        grads = []
+        for on in (False, True):
+            leaf = x.clone().requires_grad_()
+            with ops.activation_checkpoints8(least=64, enabled=on):
+                y = layer(leaf)
+            grads.append(torch.autograd.grad(y, leaf, K.seeded(y.shape, 4).to(device))[0])
+        assert torch.equal(*grads), name
+
+
+CHECKS = [check_frozen_parameters]
+
+
+@pytest.mark.parametrize("check", CHECKS, ids=lambda f: f.__name__[6:])
+def test_emulated(emu_lib, check):
+    with backend(emu_lib):
+        check("cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("check", CHECKS, ids=lambda f: f.__name__[6:])
+def test_gpu(check):
+    check("cuda:0")
