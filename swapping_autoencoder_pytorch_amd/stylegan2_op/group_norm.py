@@ -2,7 +2,7 @@
 with statistics; this stands beside ``fused_leaky_relu`` and ``plane_affine`` for networks that do."""
 import torch
 from torch import nn
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import hip_lib
@@ -82,7 +82,7 @@ def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, activati
     given).  x: float32, bfloat16 or float16, channels last in memory (any other order is copied into it); the result is channels
     last.  weight, bias: float32 [C] or None.  checkpoint: the backward pass works from the 8-bit checkpoint of x that the forward
     writes beside y, instead of from x (``checkpoint8``); y is the same, the gradients are those at the values it stands for.
-    Differentiable once."""
+    Differentiable once, in reverse mode."""
     if activation not in ACTIVATIONS:
         raise hip_lib.SaeError("group_norm_act: activation must be one of %s, got %r" % (sorted(ACTIVATIONS), activation))
     if input.dim() < 2 or input.shape[1] < 1 or num_groups < 1 or input.shape[1] % num_groups:
@@ -98,8 +98,9 @@ def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, activati
         scale = 2 ** 0.5 if activation == "lrelu" else 1.0
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    if torch.is_grad_enabled() and (input.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    # (a forward-mode level: by the Function, which refuses a tangent)
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            input.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return GroupNormActFunction.apply(input, weight, bias, num_groups, eps, ACTIVATIONS[activation], negative_slope, scale,
                                           bool(checkpoint))
     return _forward(hip_lib.get(), input, weight, bias, num_groups, eps, ACTIVATIONS[activation], negative_slope, scale, False)[0]

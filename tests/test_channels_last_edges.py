@@ -2,6 +2,7 @@
 differentiation, small gradients, the sizes on both sides of every choice between kernels."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import channels_last_cases as K
 from parity_common import backend
@@ -42,7 +43,22 @@ def check_frozen_parameters(device):
         assert torch.equal(*grads), name
 
 
-CHECKS = [check_frozen_parameters]
+def check_forward_mode(device):
+    """a tangent is refused, as by every custom function of the framework, never dropped; inside a level without tangents nothing
+    changes"""
+    x, w = K.seeded((2, 8, 3), 1).to(device), K.seeded((8,), 2).to(device)
+    want = ops.group_norm_act(x, 2, w)
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(x, torch.ones_like(x)), 2, w), (x, 2, forward_ad.make_dual(w, torch.ones_like(w))),
+                     (x, 2, None, forward_ad.make_dual(w, torch.ones_like(w)))):
+            with pytest.raises(NotImplementedError):
+                ops.group_norm_act(*args)
+            with pytest.raises(NotImplementedError), torch.no_grad():
+                ops.group_norm_act(*args)
+        assert torch.equal(ops.group_norm_act(x, 2, w), want)
+
+
+CHECKS = [check_frozen_parameters, check_forward_mode]
 
 
 @pytest.mark.parametrize("check", CHECKS, ids=lambda f: f.__name__[6:])
