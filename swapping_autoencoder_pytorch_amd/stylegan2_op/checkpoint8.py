@@ -167,7 +167,7 @@ class _Kept:
 
 
 def _pack(t, least):
-    if t.dtype not in hip_lib.element_types() or t.numel() < least or _lives_anyway(t):
+    if t.layout != torch.strided or t.dtype not in hip_lib.element_types() or t.numel() < least or _lives_anyway(t):
         return t
     if not t.is_cuda and hip_lib.get().device_only:
         return t
@@ -193,7 +193,7 @@ def _unpack(k):
 def activation_checkpoints8(least=65536, enabled=True):
     """Every autograd node built inside keeps the activations it saves (float32, bfloat16, float16; at least ``least`` values) as
     8-bit checkpoints and gets them back when its backward runs, wherever that is.  Parameters (trainable or frozen), other leaves
-    that require a gradient, views of either, small tensors and host tensors are kept as they are.  A weight that is no Parameter --
+    that require a gradient, views of either, small, sparse and host tensors are kept as they are.  A weight that is no Parameter --
     detached, or computed from one -- is an activation here.  Forward values do not change; gradients are those at the values that
     the checkpoints stand for."""
     if not enabled:

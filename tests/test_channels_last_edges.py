@@ -58,10 +58,21 @@ def check_forward_mode(device):
         assert torch.equal(ops.group_norm_act(x, 2, w), want)
 
 
+def check_other_layouts(device):
+    """a saved tensor without strides stays as it is"""
+    x = K.seeded((40, 40), 1).to(device).requires_grad_()
+    a = (K.seeded((40, 40), 2) * (K.seeded((40, 40), 3) > 0)).to(device)
+    for sparse in (a.to_sparse(), a.to_sparse_csr()):
+        with ops.activation_checkpoints8(least=64):
+            y = sparse @ (x * 1.0)
+        gx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert torch.allclose(gx, a.sum(0)[:, None].expand(40, 40), rtol=0, atol=40 * K.E32 * 40)
+
+
 CHECKS = [check_frozen_parameters, check_forward_mode]
 
 
-@pytest.mark.parametrize("check", CHECKS, ids=lambda f: f.__name__[6:])
+@pytest.mark.parametrize("check", CHECKS + [check_other_layouts], ids=lambda f: f.__name__[6:])
 def test_emulated(emu_lib, check):
     with backend(emu_lib):
         check("cpu")
