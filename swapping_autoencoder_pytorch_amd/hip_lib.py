@@ -261,8 +261,11 @@ def element_types():
 
 
 def dense(t):
-    """`t` contiguous and 16-byte aligned: itself where it is, a copy where not (a slice that starts inside a 16-byte cell)."""
+    """`t` contiguous and 16-byte aligned: itself where it is, a copy where not (a slice that starts inside a 16-byte cell, a view
+    with its sign in a flag)."""
     t = t.contiguous()
+    if t.is_neg():
+        t = t.resolve_neg()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 

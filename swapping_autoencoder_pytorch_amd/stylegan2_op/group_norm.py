@@ -14,7 +14,7 @@ ACTIVATIONS = {"none": 0, "lrelu": 1, "silu": 2}
 def _last(x):
     """(dense memory [n, ..., c] of x [n, c, ...], n, positions, c); no copy for a channels-last tensor."""
     shape = x.shape
-    if len(shape) == 4 and x.is_contiguous(memory_format=torch.channels_last) and x.data_ptr() % 16 == 0:
+    if len(shape) == 4 and x.is_contiguous(memory_format=torch.channels_last) and x.data_ptr() % 16 == 0 and not x.is_neg():
         return x, shape[0], shape[2] * shape[3], shape[1]
     return hip_lib.dense(x.movedim(1, -1)).movedim(-1, 1), shape[0], shape[2:].numel(), shape[1]
 

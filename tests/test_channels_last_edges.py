@@ -69,7 +69,21 @@ def check_other_layouts(device):
         assert torch.allclose(gx, a.sum(0)[:, None].expand(40, 40), rtol=0, atol=40 * K.E32 * 40)
 
 
-CHECKS = [check_frozen_parameters, check_forward_mode]
+def check_negative_views(device):
+    """the imaginary part of a conjugate is a view with its sign in a flag: read with the sign"""
+    z = torch.complex(K.seeded((1, 1), 1), K.seeded((1, 1), 2)).to(device)
+    x = z.conj().imag
+    assert x.is_neg() and x.is_contiguous()
+    wide = torch._neg_view(K.seeded((2, 4, 8, 8), 3).to(device).contiguous(memory_format=torch.channels_last))
+    for t in (x, wide.movedim(1, -1)):
+        assert torch.equal(ops.checkpoint8(t).dequantize(), ops.checkpoint8(t.resolve_neg().clone()).dequantize())
+    assert torch.equal(ops.group_norm_act(wide, 2), ops.group_norm_act(wide.resolve_neg(), 2))
+    rows = wide.reshape(-1, 8)
+    kept = ops.checkpoint8(rows)
+    assert torch.equal(ops.linear_weight_grad8(rows, kept)[0], ops.linear_weight_grad8(rows.resolve_neg(), kept)[0])
+
+
+CHECKS = [check_frozen_parameters, check_forward_mode, check_negative_views]
 
 
 @pytest.mark.parametrize("check", CHECKS + [check_other_layouts], ids=lambda f: f.__name__[6:])
