@@ -14,10 +14,12 @@ NaN or an infinity comes back as NaN.
 
 The reference keeps every activation in fp32 (it never enables AMP)."""
 import contextlib
+import weakref
 
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
+from torch.multiprocessing.reductions import StorageWeakRef
 
 from .. import hip_lib
 from .conv2d_gemm import _Flags, _gemm
@@ -163,14 +165,52 @@ def _lives_anyway(t):
 
 class _Kept:
     """One packed activation: the checkpoint of its memory in order, and the strides it had."""
-    __slots__ = ("kept", "size", "stride")
+    __slots__ = ("kept", "size", "stride", "__weakref__")
 
 
-def _pack(t, least):
+class _Saves:
+    """What one block of the context has packed so far, while a node holds it.  Autograd keeps ONE tensor for all the nodes that
+    save it (an activation is its own node's output and the next one's input); here those nodes share one checkpoint, or two of
+    them would take more than a 16-bit tensor itself.  A tensor is the same as long as its storage lives (the entry's weak
+    reference keeps the storage's handle, not its memory, from being used again) and its version counter stands still; what is
+    packed on one stream, or outside of a capture, is not there for another stream or inside of one."""
+    __slots__ = ("entries", "captured")
+
+    def __init__(self):
+        self.entries, self.captured = {}, self.capturing()
+
+    @staticmethod
+    def capturing():
+        return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+    def pack(self, t, build):
+        if t.is_cuda and self.capturing() != self.captured:
+            return build(t)
+        storage = t.untyped_storage()
+        key = (storage._cdata, t.storage_offset(), t.dtype, t.is_neg(), t.size(), t.stride(), t._version, hip_lib.get().stream(t))
+        entry = self.entries.get(key)
+        kept = entry[0]() if entry is not None else None
+        if kept is None:
+            kept = build(t)
+            if isinstance(kept, _Kept):
+                self.entries[key] = (weakref.ref(kept, lambda ref: self._drop(key, ref)), StorageWeakRef(storage))
+        return kept
+
+    def _drop(self, key, ref):
+        entry = self.entries.get(key)
+        if entry is not None and entry[0] is ref:
+            del self.entries[key]
+
+
+def _pack(t, least, saves):
     if t.layout != torch.strided or t.dtype not in hip_lib.element_types() or t.numel() < least or _lives_anyway(t):
         return t
     if not t.is_cuda and hip_lib.get().device_only:
         return t
+    return saves.pack(t, _keep)
+
+
+def _keep(t):
     order = sorted(range(t.dim()), key=lambda d: (-t.stride(d), d))
     flat = t.detach().permute(order)
     if not flat.is_contiguous():          # expanded, overlapping or with gaps: as it is
@@ -192,12 +232,13 @@ def _unpack(k):
 @contextlib.contextmanager
 def activation_checkpoints8(least=65536, enabled=True):
     """Every autograd node built inside keeps the activations it saves (float32, bfloat16, float16; at least ``least`` values) as
-    8-bit checkpoints and gets them back when its backward runs, wherever that is.  Parameters (trainable or frozen), other leaves
+    8-bit checkpoints and gets them back when its backward runs, wherever that is; nodes that save the same tensor share one.  Parameters (trainable or frozen), other leaves
     that require a gradient, views of either, small, sparse and host tensors are kept as they are.  A weight that is no Parameter --
     detached, or computed from one -- is an activation here.  Forward values do not change; gradients are those at the values that
     the checkpoints stand for."""
     if not enabled:
         yield
         return
-    with torch.autograd.graph.saved_tensors_hooks(lambda t: _pack(t, least), _unpack):
+    saves = _Saves()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: _pack(t, least, saves), _unpack):
         yield

@@ -83,7 +83,83 @@ def check_negative_views(device):
     assert torch.equal(ops.linear_weight_grad8(rows, kept)[0], ops.linear_weight_grad8(rows.resolve_neg(), kept)[0])
 
 
-CHECKS = [check_frozen_parameters, check_forward_mode, check_negative_views]
+def _packs(run):
+    """run() and how often it packed"""
+    lib = hip_lib.get()
+    plain, names = lib.call, []
+
+    def call(name, *args):
+        names.append(name)
+        return plain(name, *args)
+    lib.call = call
+    try:
+        return run(), names.count("checkpoint8_pack")
+    finally:
+        del lib.call
+
+
+def kept_values(t):
+    """what the context keeps of a contiguous t, in 64 bits"""
+    return K.plain_codes(t.detach().cpu().reshape(-1, 64))[2].view(t.shape)
+
+
+def check_shared(device):
+    """nodes that save the same tensor share one checkpoint; a tensor that was written in between, another view and new values in
+    the same memory have their own.  Every gradient is a sum of at most three products of kept values."""
+    x = K.seeded((64, 64), 1).to(device).requires_grad_()
+    gz = K.seeded((64, 64), 2).to(device)
+    plain = {}
+
+    def near(got, want, size):
+        assert ((got.cpu().double() - want).abs() <= 8 * K.E32 * size).all()
+
+    def shared():
+        with ops.activation_checkpoints8(least=64):
+            h = x * 1.0
+            s = torch.sigmoid(h)
+            y = h * h
+            z = s * y
+        plain.update(h=h, s=s, y=y)
+        return z
+    z, packs = _packs(shared)
+    assert packs == 3                                # h, s, y: saved five times
+    h, s, y = (kept_values(plain[n]) for n in "hsy")
+    g = gz.cpu().double()
+    gx, = torch.autograd.grad(z, x, gz)
+    near(gx, 2 * g * s * h + g * y * s * (1 - s), 2 * (g * s * h).abs() + (g * y * s).abs() * (1 + s.abs()))
+
+    def written():
+        with ops.activation_checkpoints8(least=64):
+            w = x.detach() * 1.0
+            a = x * w                                # (x is a leaf: only w is kept)
+            first = w.clone()
+            w.mul_(-3.0)
+            b = x * w
+        return a, b, first, w
+    (a, b, first, w), packs = _packs(written)
+    assert packs == 2
+    for out, want in ((a, first), (b, w)):
+        near(torch.autograd.grad(out, x, gz)[0], g * kept_values(want), (g * kept_values(want)).abs())
+
+    def views():
+        with ops.activation_checkpoints8(least=64):
+            w = x.detach() * 1.0
+            return [x[:32] * w[:32], x[32:] * w[32:], x * w, x.t() * w.t()], w
+    (outs, w), packs = _packs(views)
+    assert packs == 4
+    parts = [torch.cat([g[:32], g[:32]]) * kept_values(w), g * kept_values(w), g.t() * kept_values(w)]
+    near(sum(torch.autograd.grad(o, x, gz[:o.shape[0]] if i < 2 else gz)[0] for i, o in enumerate(outs)), sum(parts),
+         sum(t.abs() for t in parts))
+
+    # freed memory that comes back with other values
+    with ops.activation_checkpoints8(least=64):
+        outs = [x * (x.detach() * float(i)) for i in range(1, 9)]
+    for i, o in enumerate(outs):
+        want = g * kept_values(x.detach() * float(i + 1))
+        near(torch.autograd.grad(o, x, gz)[0], want, want.abs())
+
+
+CHECKS = [check_frozen_parameters, check_forward_mode, check_negative_views, check_shared]
 
 
 @pytest.mark.parametrize("check", CHECKS + [check_other_layouts], ids=lambda f: f.__name__[6:])
@@ -96,3 +172,58 @@ def test_emulated(emu_lib, check):
 @pytest.mark.parametrize("check", CHECKS, ids=lambda f: f.__name__[6:])
 def test_gpu(check):
     check("cuda:0")
+
+
+@pytest.mark.gpu
+def test_gpu_context_memory():
+    """what the context holds of an activation that two nodes save: 33 bytes for 32 values, once"""
+    for dtype, share in ((torch.float32, 33 / 128), (torch.bfloat16, 33 / 64)):
+        x = torch.randn(64, 1 << 18, device="cuda").to(dtype).requires_grad_()
+        size = x.numel() * x.element_size()
+        held = []
+        for on in (False, True):
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            with ops.activation_checkpoints8(enabled=on):
+                h = x * 1.0
+                out = (torch.sigmoid(h) * (h * h)).sum()             # h three times, its sigmoid twice, the square once
+                del h
+            torch.cuda.synchronize()
+            held.append((torch.cuda.memory_allocated() - before) / size)
+            del out
+        assert abs(held[0] - 3) < 0.01 and abs(held[1] - 3 * share) < 0.01, (dtype, held)
+
+
+@pytest.mark.gpu
+def test_gpu_shared_on_two_streams_and_captured():
+    """a tensor that is saved eagerly, on another stream and inside a capture of the same block: each replay reads what the tensor
+    holds then (the leaves of the captured and of the eager nodes are not the same)"""
+    make = lambda seed: K.seeded((256, 512), seed).cuda()
+    h, gy = make(1), make(2)
+    leaves = [make(3).requires_grad_() for _ in range(3)]
+    kept = lambda t: ops.checkpoint8(t).dequantize()
+    side, warm = torch.cuda.Stream(), torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm), ops.activation_checkpoints8(least=64):
+        torch.autograd.grad((leaves[2] * h) * h, leaves[2], gy)
+    torch.cuda.current_stream().wait_stream(warm)
+    graph = torch.cuda.CUDAGraph()
+    with ops.activation_checkpoints8(least=64):
+        eager = leaves[0] * h
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = leaves[1] * h
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            out, = torch.autograd.grad((leaves[2] * h) * h, leaves[2], gy)
+    want = kept(h) * gy
+    assert torch.equal(torch.autograd.grad(eager, leaves[0], gy)[0], want)
+    assert torch.equal(torch.autograd.grad(other, leaves[1], gy)[0], want)
+    for seed in (4, 5, 6):
+        h.copy_(make(seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        got, want = out.clone(), gy * kept(h) * kept(h)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), seed
