@@ -1,8 +1,11 @@
 """The channels-last operators at their edges: frozen weights, shared and foreign tensors inside activation_checkpoints8, forward-mode
 differentiation, small gradients, the sizes on both sides of every choice between kernels."""
+import contextlib
+
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.utils._python_dispatch import TorchDispatchMode
 
 import channels_last_cases as K
 from parity_common import backend
@@ -159,7 +162,34 @@ def check_shared(device):
         near(torch.autograd.grad(o, x, gz)[0], want, want.abs())
 
 
-CHECKS = [check_frozen_parameters, check_forward_mode, check_negative_views, check_shared]
+class _Reductions(TorchDispatchMode):
+    """torch's own sums, which put nodes into a captured graph that do not replay reliably"""
+
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        if func.overloadpacket in (torch.ops.aten.sum, torch.ops.aten.mean):
+            self.seen.append(func)
+        return func(*args, **(kwargs or {}))
+
+
+def check_linear8_bias_alone(device):
+    """the bias gradient beside a frozen weight and under input_grads_only: the framework's own sum of the rows"""
+    for rows in (0, 1, 70, 5000):
+        x, w = K.seeded((rows, 36), 1).to(device), K.seeded((20, 36), 2).to(device)
+        b, gy = K.seeded((20,), 3).to(device).requires_grad_(), K.seeded((rows, 20), 4).to(device)
+        g = gy.cpu().double()
+        for frozen in (True, False):
+            y = ops.linear8(x, w if frozen else w.clone().requires_grad_(), b)
+            with _Reductions() as torchs, (contextlib.nullcontext() if frozen else ops.input_grads_only()):
+                gb, = torch.autograd.grad(y, b, gy)
+            assert not torchs.seen
+            assert ((gb.cpu().double() - g.sum(0)).abs() <= 2 * K.E32 * (rows + 32) * g.abs().sum(0)).all()
+
+
+CHECKS = [check_frozen_parameters, check_forward_mode, check_negative_views, check_shared, check_linear8_bias_alone]
 
 
 @pytest.mark.parametrize("check", CHECKS + [check_other_layouts], ids=lambda f: f.__name__[6:])
