@@ -551,7 +551,7 @@ int sae_group_norm_act_bwd(const void* gy, const void* x, const int8_t* codes, c
 
 /* Weight gradient of a linear layer from its input's 8-bit checkpoint (csrc/linear_wgrad8.hip):
  *   gw[o][i] = alpha * sum over r of gy[r][o] * x8[r][i]   [out][c],     gb[o] = sum over r of gy[r][o]   (gb may be NULL)
- * gy, gw, gb in the element type; products exact, sums fp32.  workspace: sae_linear_wgrad8_workspace floats; it, gy and codes
+ * gy, gw, gb in the element type; products exact (SAE_F32: of values of gy below 2^-110 less than 2^-132 is lost), sums fp32.  workspace: sae_linear_wgrad8_workspace floats; it, gy and codes
  * 16-byte aligned. */
 int64_t sae_linear_wgrad8_workspace(int64_t rows, int64_t out, int64_t c, int32_t dtype);
 int sae_linear_wgrad8(const void* gy, const int8_t* codes, const uint8_t* scales, void* gw, void* gb, int64_t rows, int64_t out,

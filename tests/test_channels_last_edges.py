@@ -257,3 +257,41 @@ def test_gpu_shared_on_two_streams_and_captured():
         got, want = out.clone(), gy * kept(h) * kept(h)
         torch.cuda.synchronize()
         assert torch.equal(got, want), seed
+
+
+# ---- small gradients, and values next to the ends of a type's range ------------------------------------------------------------
+
+def _wgrad_near(device, x, gy, dtype, less):
+    """linear_weight_grad8 against 64 bits.  Every fp32 addition is off by one step at most; outputs are rounded once, at least to
+    the last place of the type's subnormals; `less`: how far a value of gy may be off before it is multiplied"""
+    kept = ops.checkpoint8(x.to(device))
+    gw, gb = (t.cpu().double() for t in ops.linear_weight_grad8(gy.to(device), kept))
+    v, g, rows = K.plain_codes(x)[2], gy.double(), x.shape[0]
+    u, last = K.half_step(dtype), torch.finfo(dtype).smallest_normal * K.half_step(dtype)
+    for got, want, size, slack in ((gw, g.t() @ v, g.abs().t() @ v.abs(), less * v.abs().sum(0)),
+                                   (gb, g.sum(0), g.abs().sum(0), torch.zeros(()))):
+        bound = (2 * K.E32 * (rows + 32) * size + rows * 2.0 ** -149 + slack) * (1 + u) + u * want.abs() + last
+        assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+def check_small_gradients(device, dtype, scale):
+    for rows, c, out in ((70, 40, 33), (300, 64, 129)):
+        x, gy = K.seeded((rows, c), 1, dtype, 0.2), K.seeded((rows, out), 2, dtype, 0.0, scale)
+        # f32: pieces of bf16, whose last place is 2^-133: the two lower ones are cut there, less than a place each
+        _wgrad_near(device, x, gy, dtype, 2.0 ** -132 if dtype == torch.float32 else 0.0)
+
+
+SMALL = [("f16", 1e-3), ("f16", 1e-5), ("f16", 3e-7), ("bf16", 1e-20), ("bf16", 1e-38), ("f32", 1e-20), ("f32", 1e-32), ("f32", 1e-36),
+         ("f32", 1e-38), ("f32", 1e-40)]
+
+
+@pytest.mark.parametrize("dtype,scale", SMALL)
+def test_small_gradients_emulated(emu_lib, dtype, scale):
+    with backend(emu_lib):
+        check_small_gradients("cpu", K.TYPES[dtype], scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,scale", SMALL)
+def test_gpu_small_gradients(dtype, scale):
+    check_small_gradients("cuda:0", K.TYPES[dtype], scale)
