@@ -295,3 +295,180 @@ def test_small_gradients_emulated(emu_lib, dtype, scale):
 @pytest.mark.parametrize("dtype,scale", SMALL)
 def test_gpu_small_gradients(dtype, scale):
     check_small_gradients("cuda:0", K.TYPES[dtype], scale)
+
+
+# ---- the norm's kernels on both sides of every choice between them, against 64 bits --------------------------------------------
+
+def norm_near(device, dtype, shape, act, checkpoint, mean=0.5, count=64, affine=True):
+    """group_norm_act and its backward against the formulas in 64 bits on the same device.  count: a thread's rows, the steps of
+    its work-group's fold and the roundings behind -- what is added in fp32 one after the other (records are added in 64 bits)"""
+    n, space, c, groups = shape
+    full, slope = (n, c) + tuple(space), 0.2
+    wide = (1, c) + (1,) * len(space)
+    x = ((K.seeded(full, 10) + mean) * (0.5 + K.seeded((c,), 11).abs()).view(wide)).to(dtype).to(device)
+    gy = K.seeded(full, 12, dtype, 0.02, 0.1).to(device)
+    x, gy = (t.movedim(1, -1).contiguous().movedim(-1, 1) for t in (x, gy))
+    leaves = [x.requires_grad_()]
+    if affine:
+        leaves += [(1 + 0.3 * K.seeded((c,), 13)).to(device).requires_grad_(), (0.2 * K.seeded((c,), 14)).to(device).requires_grad_()]
+    y = ops.group_norm_act(*[leaves[0], groups] + leaves[1:], activation=act, negative_slope=slope, checkpoint=checkpoint)
+    grads = torch.autograd.grad(y, leaves, gy)
+    x = x.detach()
+    kept = ops.checkpoint8(x.movedim(1, -1)).dequantize().movedim(-1, 1) if checkpoint else x
+
+    split = lambda t: t.double().reshape(n, groups, c // groups, -1)
+    x64, k64, g64 = split(x), split(kept), split(gy)
+    w, b = ((t.detach().double().view(1, groups, -1, 1) for t in leaves[1:]) if affine else
+            (torch.ones((), dtype=torch.float64, device=device), torch.zeros((), dtype=torch.float64, device=device)))
+    scale = 2 ** 0.5 if act == "lrelu" else 1.0
+    over = lambda t: t.mean((2, 3), keepdim=True)
+    mu = over(x64)
+    rstd = (over((x64 - mu) ** 2) + 1e-5) ** -0.5
+    e = K.E32
+    z = (x64 - mu) * rstd * w + b
+    offset = mu.abs() * rstd                                    # the mean is rounded to fp32
+    # the variance: sums of (x - x0)^2, off by `count` steps of a sum at most (2 + the distance of x0)^2 larger; rstd by half of that
+    spread = count * e * (2 + ((x64 - mu).abs() * rstd).amax((2, 3), keepdim=True)) ** 2
+    ey = scale * ((16 * e + spread) * w.abs() * (x64 - mu).abs() * rstd + 16 * e * (w.abs() * offset + b.abs()) + 8 * e) * (1 + z.abs())
+    xh = (k64 - mu) * rstd
+    zk = xh * w + b
+    dz = g64 * scale * K.act_slope64(zk, act, slope)
+    ez = (16 * e + spread) * w.abs() * xh.abs() + 16 * e * (w.abs() * offset + b.abs())
+    ed = (g64 * scale).abs() * (16 * e * (1 + zk.abs()) + (ez if act == "silu" else 0.0))
+    if act == "lrelu":                                          # on either side of the kink
+        ed = ed + torch.where(zk.abs() <= ez, (1 - slope) * (g64 * scale).abs(), torch.zeros_like(ed))
+    exh = (8 * e + spread) * xh.abs() + 8 * e * offset
+    wd = w * dz
+    m1, m2 = over(wd), over(wd * xh)
+    em1 = over(w.abs() * ed) + count * e * over(wd.abs())
+    em2 = over(w.abs() * ed * xh.abs() + wd.abs() * exh) + count * e * over((wd * xh).abs())
+    egx = rstd * (w.abs() * ed + em1 + exh * m2.abs() + xh.abs() * em2 + (8 * e + spread) * (wd.abs() + m1.abs() + (xh * m2).abs()))
+    total = lambda t: t.sum((0, 3)).view(-1)
+    u = K.half_step(dtype)
+    checks = [("y", y.detach(), scale * K.act64(z, act, slope), ey, u), ("gx", grads[0], rstd * (wd - m1 - xh * m2), egx, u)]
+    if affine:
+        checks += [("gw", grads[1], total(dz * xh), total(ed * xh.abs() + dz.abs() * exh + count * e * (dz * xh).abs()), e),
+                   ("gb", grads[2], total(dz), total(ed + count * e * dz.abs()), e)]
+    for name, got, want, bound, u in checks:
+        off = (got.double().reshape(want.shape) - want).abs()
+        bound = bound * (1 + u) + u * want.abs() + torch.finfo(dtype).smallest_normal * u
+        assert (off <= bound).all(), (name, shape, act, checkpoint, float((off / bound).max()))
+
+
+# one launch; folded totals in both directions; three launches; more channels than are folded, wide groups, one group, ragged channels
+# and groups; sizes on both sides of the one-launch rule (10 MB forward, 4 MB backward)
+BORDERS = [(2, (64, 64), 512, 32), (4, (128, 128), 128, 32), (3, (33, 65), 100, 20), (5, (17, 129), 72, 8), (2, (128, 128), 64, 1),
+           (2, (40, 50), 1030, 2), (1, (300, 301), 48, 2), (16, (31, 33), 128, 32), (16, (32, 32), 128, 32), (8, (70, 71), 64, 8),
+           (2, (9, 9), 2048, 4), (1, (200, 200), 5, 5), (40, (3, 5), 512, 512), (6, (90, 90), 96, 3)]
+
+
+@pytest.mark.parametrize("dtype", sorted(K.TYPES))
+def test_norm_near_emulated(emu_lib, dtype, monkeypatch):
+    """the same check on the sources, each form of launch at small sizes"""
+    with backend(emu_lib):
+        for one, fold in (("1", "1"), ("0", "1"), ("0", "0")):
+            monkeypatch.setenv("SAE_GN_ONE_LAUNCH", one)
+            monkeypatch.setenv("SAE_GN_FOLD", fold)
+            for act, checkpoint, mean in (("silu", False, 0.5), ("lrelu", True, -3.0), ("none", False, 100.0)):
+                norm_near("cpu", K.TYPES[dtype], (2, (13, 27), 40, 4), act, checkpoint, mean, affine=act != "none")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", BORDERS, ids=lambda s: "n%d_%s_c%d_g%d" % (s[0], "x".join(map(str, s[1])), s[2], s[3]))
+@pytest.mark.parametrize("dtype", sorted(K.TYPES))
+def test_gpu_norm_near(dtype, shape):
+    norm_near("cuda:0", K.TYPES[dtype], shape, "silu", False)
+    norm_near("cuda:0", K.TYPES[dtype], shape, "silu", True, mean=-3.0)
+    norm_near("cuda:0", K.TYPES[dtype], shape, "lrelu", False, mean=0.0)
+    norm_near("cuda:0", K.TYPES[dtype], shape, "none", True, mean=100.0, affine=False)
+
+
+# ---- infinities and NaN at every tile height of the weight gradient ------------------------------------------------------------
+
+def check_wgrad_not_finite(device, dtype, shape):
+    """single values that are not finite, in gy and in x, at both ends and in the middle of the rows: every output that does not
+    meet one is as near as ever, every other one the infinity or NaN that IEEE arithmetic gives"""
+    rows, c, out = shape
+    x, gy = K.seeded((rows, c), 1, dtype, 0.2), K.seeded((rows, out), 2, dtype, 0.0, 0.3)
+    for i, value in enumerate((float("inf"), float("-inf"), float("nan"))):
+        gy[(0, rows // 2, rows - 1)[i], (5 + 61 * i) % out] = value
+    gy[rows // 3, 0], gy[rows // 3 + 1, 0] = float("inf"), float("-inf")
+    x[rows // 2, c - 1], x[rows - 1, 0] = float("nan"), float("inf")       # whole blocks of 32 channels
+    kept = ops.checkpoint8(x.to(device))
+    gw, gb = ops.linear_weight_grad8(gy.to(device), kept)
+    v, g = kept.dequantize().double(), gy.to(device).double().t().contiguous()
+    for got, want, size in ((gw.double(), g @ v, g.abs() @ v.abs()), (gb.double(), g.sum(1), g.abs().sum(1))):
+        fine, u = torch.isfinite(want), K.half_step(dtype)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+        assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)]) and not fine.all()
+        assert c <= 64 or fine.any()                                       # (of two blocks none is left)
+        off, bound = (got - want).abs(), 2 * K.E32 * (rows + 32) * size * (1 + u) + u * want.abs()
+        assert (off <= bound)[fine].all()
+
+
+@pytest.mark.parametrize("tile", [64, 128, 256])
+@pytest.mark.parametrize("dtype", sorted(K.TYPES))
+def test_wgrad_not_finite_emulated(emu_lib, dtype, tile, monkeypatch):
+    monkeypatch.setenv("SAE_WG_TILE", str(tile))
+    with backend(emu_lib):
+        for shape in ((70, 130, 300), (330, 64, 140)):
+            check_wgrad_not_finite("cpu", K.TYPES[dtype], shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(300, 130, 70), (40000, 130, 100), (40000, 200, 300), (33000, 100, 2048)], ids=lambda s: "r%d_c%d_o%d" % s)
+@pytest.mark.parametrize("dtype", sorted(K.TYPES))
+def test_gpu_wgrad_not_finite(dtype, shape):
+    """sizes that take each tile height by themselves"""
+    check_wgrad_not_finite("cuda:0", K.TYPES[dtype], shape)
+
+
+# ---- the framework's own layers inside the context ------------------------------------------------------------------------------
+
+def check_layers_in_context(device):
+    """with trainable weights too the input gradient of a layer is the plain one bit for bit (weights as they are, masks by sign),
+    and the weight gradient of a product is the one at what is kept of its input, bit for bit"""
+    for name, layer, params, shape in _layers(device):
+        x, kept = K.seeded(shape, 3).to(device).requires_grad_(), None
+        both = []
+        for on in (False, True):
+            with ops.activation_checkpoints8(least=64, enabled=on):
+                y = layer(x)
+            both.append(torch.autograd.grad(y, x, K.seeded(y.shape, 4).to(device))[0])
+        assert torch.equal(*both), name
+        if name in ("ConvLayer", "ResBlock"):
+            continue
+        h = x.detach() * 1.0
+        width = next((w for w in (4096, 512, 64, 32) if h.numel() % w == 0), h.numel())
+        kept = ops.checkpoint8(h.reshape(-1, width)).dequantize().view(h.shape)
+        gy = K.seeded(y.shape, 5).to(device)
+        with ops.activation_checkpoints8(least=64):
+            y = layer(h)
+        got = torch.autograd.grad(y, params[0], gy)[0]
+        if name == "EqualLinear":                               # (the mask is that of the values before they were kept)
+            gy = gy * torch.where(y.detach() > 0, 1.0, 0.2) * 2 ** 0.5
+            plain = ops.linear(kept, params[0], None, layer.scale)
+        else:
+            plain = layer(kept)
+        want = torch.autograd.grad(plain, params[0], gy)[0]
+        if name == "EqualLinear":
+            g = gy.cpu().double()
+            size = layer.scale * g.abs().t() @ kept.cpu().double().abs()
+            assert ((got - want).cpu().double().abs() <= 2 * 8 * K.E32 * size).all(), name
+        else:
+            assert torch.equal(got, want), name
+
+
+IN_LAYERS = [check_layers_in_context]
+
+
+@pytest.mark.parametrize("check", IN_LAYERS, ids=lambda f: f.__name__[6:])
+def test_layers_emulated(emu_lib, check):
+    with backend(emu_lib):
+        check("cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("check", IN_LAYERS, ids=lambda f: f.__name__[6:])
+def test_gpu_layers(check):
+    check("cuda:0")
