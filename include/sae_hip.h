@@ -539,7 +539,7 @@ int sae_checkpoint8_unpack(const int8_t* codes, const uint8_t* scales, void* x, 
  *                           n * l = 0 gw and gb are zero).  From a checkpoint the gradients are those at the values it stands for,
  *                           with the statistics of the forward pass.
  *   sae_group_norm_act_workspace   bytes of workspace either needs (backward = 0 / 1)
- * Tensors and workspace 16-byte aligned, n <= 65535.  Sums are added in a fixed order (no atomics). */
+ * Tensors and workspace 16-byte aligned, n and groups <= 65535, c <= 2^20, n * l * c <= 2^40.  Sums are added in a fixed order (no atomics). */
 int64_t sae_group_norm_act_workspace(int64_t n, int64_t l, int64_t c, int64_t groups, int32_t dtype, int32_t backward);
 int sae_group_norm_act(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd, int8_t* codes,
                        uint8_t* scales, int64_t n, int64_t l, int64_t c, int64_t groups, float eps, int32_t act, float slope,
@@ -551,8 +551,8 @@ int sae_group_norm_act_bwd(const void* gy, const void* x, const int8_t* codes, c
 
 /* Weight gradient of a linear layer from its input's 8-bit checkpoint (csrc/linear_wgrad8.hip):
  *   gw[o][i] = alpha * sum over r of gy[r][o] * x8[r][i]   [out][c],     gb[o] = sum over r of gy[r][o]   (gb may be NULL)
- * gy, gw, gb in the element type; products exact (SAE_F32: of values of gy below 2^-110 less than 2^-132 is lost), sums fp32.  workspace: sae_linear_wgrad8_workspace floats; it, gy and codes
- * 16-byte aligned. */
+ * gy, gw, gb in the element type; products exact (SAE_F32: of values of gy below 2^-110 less than 2^-132 is lost), sums
+ * fp32.  workspace: sae_linear_wgrad8_workspace floats; it, gy and codes 16-byte aligned. */
 int64_t sae_linear_wgrad8_workspace(int64_t rows, int64_t out, int64_t c, int32_t dtype);
 int sae_linear_wgrad8(const void* gy, const int8_t* codes, const uint8_t* scales, void* gw, void* gb, int64_t rows, int64_t out,
                       int64_t c, float alpha, int32_t dtype, float* workspace, int64_t workspace_floats, sae_stream_t stream);

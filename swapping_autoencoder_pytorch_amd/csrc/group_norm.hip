@@ -865,9 +865,16 @@ __global__ __launch_bounds__(kFused) void gn_bwd_fused_kernel(const typename Ele
 
 constexpr int64_t kMostChannels = 1 << 20, kMostSamples = 65535;
 
-bool gn_shape_ok(int64_t n, int64_t l, int64_t c, int64_t groups) {
-    return n >= 0 && n <= kMostSamples && l >= 0 && c >= 1 && c <= kMostChannels && groups >= 1 && groups <= 65535 &&
-           c % groups == 0 && l <= ((int64_t)1 << 40) / c;
+constexpr int64_t kMostValues = (int64_t)1 << 40;
+
+// what a shape breaks (nullptr: nothing).  Samples are the grid's second dimension; a chunk's rows and its records are counted in 32 bits
+const char* gn_shape_fault(int64_t n, int64_t l, int64_t c, int64_t groups) {
+    if (n < 0 || l < 0 || c < 1 || groups < 1 || c % groups != 0) return "bad shape (n, l >= 0; c a multiple of groups >= 1)";
+    if (n > kMostSamples) return "more than 65535 samples";
+    if (c > kMostChannels) return "more than 1048576 channels";
+    if (groups > 65535) return "more than 65535 groups";
+    if (l > kMostValues / c || n * l > kMostValues / c) return "more than 2^40 values";
+    return nullptr;
 }
 
 // Groups of a one-launch work-group: at least 64 bytes of a row (one group's share is often less, and every 64-byte piece is read
@@ -1072,7 +1079,7 @@ int gn_dispatch(const char* what, GnArgs& a, int64_t l, int64_t c, int64_t group
 using namespace sae;
 
 extern "C" int64_t sae_group_norm_act_workspace(int64_t n, int64_t l, int64_t c, int64_t groups, int32_t dtype, int32_t backward) {
-    if (!gn_shape_ok(n, l, c, groups) || !elem_known(dtype) || n == 0 || l == 0) return 0;
+    if (gn_shape_fault(n, l, c, groups) || !elem_known(dtype) || n == 0 || l == 0) return 0;
     const int64_t without = gn_workspace(gn_plan(n, l, c, groups, elem_bytes(dtype), kNoCodes, backward != 0), n, backward != 0);
     const int64_t with = gn_workspace(gn_plan(n, l, c, groups, elem_bytes(dtype), backward ? kReadCodes : kWriteCodes, backward != 0), n,
                                        backward != 0);
@@ -1086,7 +1093,8 @@ extern "C" int sae_group_norm_act(const void* x, const float* weight, const floa
     sae::clear_stale_error();
     if (!elem_known(dtype) || act < SAE_ACT_NONE || act > SAE_ACT_SILU)
         return fail(SAE_EINVAL, "sae_group_norm_act: unknown element type or activation");
-    if (!gn_shape_ok(n, l, c, groups) || !(eps >= 0.0f)) return fail(SAE_EINVAL, "sae_group_norm_act: bad shape or eps");
+    if (const char* fault = gn_shape_fault(n, l, c, groups)) return fail(SAE_EINVAL, "sae_group_norm_act: %s", fault);
+    if (!(eps >= 0.0f)) return fail(SAE_EINVAL, "sae_group_norm_act: negative eps");
     if ((codes == nullptr) != (scales == nullptr)) return fail(SAE_EINVAL, "sae_group_norm_act: codes and scales go together");
     if (n == 0 || l == 0) return SAE_OK;
     if (!x || !y || !mean || !rstd) return fail(SAE_EINVAL, "sae_group_norm_act: null tensor");
@@ -1102,7 +1110,7 @@ extern "C" int sae_group_norm_act_bwd(const void* gy, const void* x, const int8_
     sae::clear_stale_error();
     if (!elem_known(dtype) || act < SAE_ACT_NONE || act > SAE_ACT_SILU)
         return fail(SAE_EINVAL, "sae_group_norm_act_bwd: unknown element type or activation");
-    if (!gn_shape_ok(n, l, c, groups)) return fail(SAE_EINVAL, "sae_group_norm_act_bwd: bad shape");
+    if (const char* fault = gn_shape_fault(n, l, c, groups)) return fail(SAE_EINVAL, "sae_group_norm_act_bwd: %s", fault);
     if ((codes == nullptr) != (scales == nullptr) || (codes == nullptr) == (x == nullptr && n > 0 && l > 0))
         return fail(SAE_EINVAL, "sae_group_norm_act_bwd: either x or codes and scales");
     if (n == 0 || l == 0) {

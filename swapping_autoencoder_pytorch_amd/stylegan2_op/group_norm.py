@@ -76,7 +76,7 @@ class GroupNormActFunction(Function):
 def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, activation="lrelu", negative_slope=0.2, scale=None,
                    checkpoint=False):
     """scale * act((x - mean) * rstd * weight + bias) of x [N, C, ...], mean and variance over each sample's C / num_groups
-    channels and all of its positions.
+    channels and all of its positions.  Up to 65535 samples and groups and 2 ** 20 channels; what exceeds them is refused.
 
     activation: "lrelu" (negative_slope; scale 2 ** 0.5 unless given, as ``fused_leaky_relu``), "silu" or "none" (scale 1 unless
     given).  x: float32, bfloat16 or float16, channels last in memory (any other order is copied into it); the result is channels

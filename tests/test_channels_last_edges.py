@@ -189,10 +189,30 @@ def check_linear8_bias_alone(device):
             assert ((gb.cpu().double() - g.sum(0)).abs() <= 2 * K.E32 * (rows + 32) * g.abs().sum(0)).all()
 
 
+def check_sizes_refused(device):
+    """what one launch's grid and 32-bit chunks do not hold is refused by name, in the call and at the C entries"""
+    x = torch.zeros(1, 1, device=device)
+    for shape, groups, word in (((65536, 1), 1, "65535"), ((1, (1 << 20) + 1), 1, "1048576"), ((1, 65536), 65536, "65535")):
+        with pytest.raises(hip_lib.SaeError, match=word):
+            ops.group_norm_act(x.expand(shape), groups)
+    lib = hip_lib.get()
+    fit = torch.zeros(64, device=device)
+    p = fit.data_ptr()
+    for n, l, c, groups, word in ((65536, 1, 1, 1, "65535"), (4096, 1 << 31, 1, 1, "2\\^40"), (1, 1 << 41, 1, 1, "2\\^40"),
+                                  (2, 2, 6, 4, "groups"), (1, 1, (1 << 20) + 1, 1, "1048576")):
+        with pytest.raises(hip_lib.SaeError, match=word):
+            lib.call("group_norm_act", p, None, None, p, p, p, None, None, n, l, c, groups, 1e-5, 0, 0.2, 1.0, 0, p, 64, None)
+        with pytest.raises(hip_lib.SaeError, match=word):
+            lib.call("group_norm_act_bwd", p, p, None, None, p, p, None, None, p, None, None, n, l, c, groups, 0, 0.2, 1.0, 0, p, 64, None)
+        assert lib.query("group_norm_act_workspace", n, l, c, groups, 0, 1) == 0
+    with pytest.raises(hip_lib.SaeError, match="eps"):
+        lib.call("group_norm_act", p, None, None, p, p, p, None, None, 1, 1, 1, 1, -1.0, 0, 0.2, 1.0, 0, p, 64, None)
+
+
 CHECKS = [check_frozen_parameters, check_forward_mode, check_negative_views, check_shared, check_linear8_bias_alone]
 
 
-@pytest.mark.parametrize("check", CHECKS + [check_other_layouts], ids=lambda f: f.__name__[6:])
+@pytest.mark.parametrize("check", CHECKS + [check_other_layouts, check_sizes_refused], ids=lambda f: f.__name__[6:])
 def test_emulated(emu_lib, check):
     with backend(emu_lib):
         check("cpu")
