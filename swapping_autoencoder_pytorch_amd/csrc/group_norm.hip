@@ -902,14 +902,18 @@ GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int esize, GnCo
     p.units = p.cg % v == 0 ? (int)c / v : (int)c;
     p.slab = gn_slab(c, groups, v, esize, codes);
     p.slabs = p.slab ? (int)ceil_div64(groups, p.slab) : 0;
-    // One launch where a thread of kFused has at most 64 values of its slab (backward: 32) and the tensor is small.  Against three
-    // (two) launches, n of 1 ... 64, c of 96 ... 512, f32 and bf16:    forward, <= 10 MB: 16 values -30 ... -47 %, 40 -10 ... -38 %,
-    // 64 -37 ... +4 %, 128 (bf16) +22 ... +43 %; 12 to 18 MB -11 ... +21 %, 32 MB +17 ... +26 %.    backward, <= 4 MB: 8 or 16 values
-    // -43 ... -5 %, 20 -22 ... +3 %, 32 -11 ... +10 % (and a launch or two fewer), 40 -6 ... +17 %; 8 MB -8 ... +10 %, 16 MB +16 %.
+    // One launch where a thread of kFused has at most 64 values of its slab (backward: 32) and the tensor is small; backward of groups of
+    // up to 16 channels only, which one thread adds up at the end.  Time against that of two or three launches, captured, f32 and bf16,
+    // n of 1 ... 32, c of 128 ... 512 in groups of 4 ... 512, 546 shapes:
+    //   forward, <= 10 MB    values a thread   < 16: 0.54 ... 0.94     16, 32: 0.60 ... 0.94     64: 0.66 ... 1.22, median 1.0 (a launch fewer)
+    //                        (any group: one of 512 channels 0.73 ... 1.11);  beyond: 128 values 1.22 ... 1.43, 12 to 18 MB 0.89 ... 1.21
+    //   backward, <= 4 MB, up to 32 values      groups of 4: 0.11 ... 0.98     8: 0.12 ... 1.03     16: 0.15 ... 1.14
+    //                        32 channels 0.18 ... 1.28, 64 0.26 ... 1.93, 128 0.40 ... 2.83, 512 1.29 ... 7.2;  beyond 4 MB 0.92 ... 1.16
     // (knob 0, for tests: never)
     if (p.slab) {
         const int64_t values = l * p.slab * p.cg, bytes = n * l * c * esize;
-        const bool small = backward ? values <= kFused * 32 && bytes <= ((int64_t)4 << 20) : values <= kFused * 64 && bytes <= ((int64_t)10 << 20);
+        const bool small = backward ? p.cg <= 16 && values <= kFused * 32 && bytes <= ((int64_t)4 << 20)
+                                    : values <= kFused * 64 && bytes <= ((int64_t)10 << 20);
         if (!small || tuning_knob("SAE_GN_ONE_LAUNCH", 1) == 0) p.slab = 0;
     }
     // lanes of so many channels; a walk that writes codes has all lanes of a block
@@ -960,9 +964,11 @@ struct GnArgs {
     hipStream_t stream;
 };
 
-// The apply kernel adds a sample's records (`bytes` of them) itself: up to 64 KB for each work-group and 32 MB for all.  The GPU takes as
-// long either way (f16 [3, 100, 33, 65] 17.8 + 19.4 against 18.2 + 19.5 us; bf16 [2, 64, 128, 128] in one group 12.3 + 22.2 against
-// 10.9 + 16.9; at 128 KB f16 [8, 320, 1000] 18.5 against 26.2 back), a training step of two launches fewer 4 % less (139 against 133 us).
+// The apply kernel adds a sample's records (`bytes` of them) itself: up to 64 KB for each work-group and 32 MB for all.  Captured, forward
+// / backward, against a launch for the totals: few groups gain (bf16 [2, 64, 128, 128] in one group 10.8 / 17.2 against 14.5 / 22.6 us,
+// f16 [3, 100, 33, 65] in one 21.2 / 19.0 against 29.4 / 21.1, in 25 17.8 / 18.9 against 17.2 / 18.8), the most that is lost is 6 %
+// (bf16 [2, 64, 128, 128] in 16: 17.6 / 17.2 against 17.6 / 16.2); an eager training step of two launches fewer takes 4 % less.  At 128 KB
+// it takes longer (f16 [8, 320, 1000] backward 26.2 against 18.5).
 // (knob 0, for tests: never)
 bool fold_totals(const GnShape& p, int64_t n, int64_t bytes) {
     return p.groups <= kFoldGroups && bytes <= ((int64_t)64 << 10) && bytes * p.chunks * n <= ((int64_t)32 << 20) &&

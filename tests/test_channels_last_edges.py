@@ -379,7 +379,8 @@ def norm_near(device, dtype, shape, act, checkpoint, mean=0.5, count=64, affine=
 # and groups; sizes on both sides of the one-launch rule (10 MB forward, 4 MB backward)
 BORDERS = [(2, (64, 64), 512, 32), (4, (128, 128), 128, 32), (3, (33, 65), 100, 20), (5, (17, 129), 72, 8), (2, (128, 128), 64, 1),
            (2, (40, 50), 1030, 2), (1, (300, 301), 48, 2), (16, (31, 33), 128, 32), (16, (32, 32), 128, 32), (8, (70, 71), 64, 8),
-           (2, (9, 9), 2048, 4), (1, (200, 200), 5, 5), (40, (3, 5), 512, 512), (6, (90, 90), 96, 3)]
+           (2, (9, 9), 2048, 4), (1, (200, 200), 5, 5), (40, (3, 5), 512, 512), (6, (90, 90), 96, 3), (2, (16, 16), 128, 2),
+           (2, (16, 16), 512, 1), (4, (15, 16), 256, 16)]
 
 
 @pytest.mark.parametrize("dtype", sorted(K.TYPES))
@@ -391,6 +392,15 @@ def test_norm_near_emulated(emu_lib, dtype, monkeypatch):
             monkeypatch.setenv("SAE_GN_FOLD", fold)
             for act, checkpoint, mean in (("silu", False, 0.5), ("lrelu", True, -3.0), ("none", False, 100.0)):
                 norm_near("cpu", K.TYPES[dtype], (2, (13, 27), 40, 4), act, checkpoint, mean, affine=act != "none")
+
+
+def test_wide_groups_take_more_launches(emu_lib):
+    """the backward pass in one launch is for groups that one thread adds up: with a workspace (records of chunks) from 17 channels"""
+    for c, groups, one in ((512, 32, True), (512, 30, None), (512, 16, False), (128, 1, False), (34, 2, False), (32, 2, True)):
+        if one is None:
+            assert emu_lib.query("group_norm_act_workspace", 1, 16, c, groups, 0, 1) == 0        # (no such shape)
+        else:
+            assert (emu_lib.query("group_norm_act_workspace", 1, 16, c, groups, 0, 1) == 0) == one, (c, groups)
 
 
 @pytest.mark.gpu
