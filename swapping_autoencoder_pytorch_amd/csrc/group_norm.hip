@@ -907,8 +907,8 @@ GnShape gn_plan(int64_t n, int64_t l, int64_t c, int64_t groups, int esize, GnCo
     // n of 1 ... 32, c of 128 ... 512 in groups of 4 ... 512, 546 shapes:
     //   forward, <= 10 MB    values a thread   < 16: 0.54 ... 0.94     16, 32: 0.60 ... 0.94     64: 0.66 ... 1.22, median 1.0 (a launch fewer)
     //                        (any group: one of 512 channels 0.73 ... 1.11);  beyond: 128 values 1.22 ... 1.43, 12 to 18 MB 0.89 ... 1.21
-    //   backward, <= 4 MB, up to 32 values      groups of 4: 0.11 ... 0.98     8: 0.12 ... 1.03     16: 0.15 ... 1.14
-    //                        32 channels 0.18 ... 1.28, 64 0.26 ... 1.93, 128 0.40 ... 2.83, 512 1.29 ... 7.2;  beyond 4 MB 0.92 ... 1.16
+    //   backward, <= 4 MB, up to 32 values   groups of 4 channels 0.51 ... 0.99, 8 0.57 ... 1.02, 16 0.69 ... 1.13; of 32 11 ... 20 us, 64
+    //                        16 ... 25, 128 27 ... 34, 256 48 ... 57, against 10 ... 17 in more launches
     // (knob 0, for tests: never)
     if (p.slab) {
         const int64_t values = l * p.slab * p.cg, bytes = n * l * c * esize;
@@ -1027,7 +1027,11 @@ void gn_backward_as(const GnArgs& a, const GnShape& p) {
     float2* means = totals + a.n * p.c;
     hipLaunchKernelGGL((gn_bwd_sums_kernel<DT, ANY, ACT, KEPT>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
                        (const int8_t*)a.codes, (const uint8_t*)a.scales, in, rec, a.slope, p);
-    if (p.c <= kFoldChannels && fold_totals(p, a.n, (int64_t)p.chunks * p.c * (int64_t)sizeof(float2))) {
+    // (a wave adds two channels' weight gradients at most: where few work-groups share many channels, that is what everything waits
+    // for -- f32 [1, 512, 4, 4] 49 us against 12 with a launch for the totals, [1, 128, 8, 8] 20 against 12, [4, 256, 8, 8], four
+    // channels a wave, 13 against 12; two: [8, 256, 8, 8] 11 against 13, bf16 [4, 128, 32, 32] 14 against 16)
+    const bool waves = p.c <= 2 * (kBlock / kWave) * (int64_t)p.chunks * a.n;
+    if (waves && p.c <= kFoldChannels && fold_totals(p, a.n, (int64_t)p.chunks * p.c * (int64_t)sizeof(float2))) {
         hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, ANY, ACT, KEPT, true>), grid, block, 0, a.stream, (const T*)a.gy, (const T*)a.x,
                            (const int8_t*)a.codes, (const uint8_t*)a.scales, in, (const float2*)rec, (const float2*)nullptr,
                            (const float2*)nullptr, a.gw, a.gb, (T*)a.out, a.slope, a.scale, p);

@@ -380,7 +380,8 @@ def norm_near(device, dtype, shape, act, checkpoint, mean=0.5, count=64, affine=
 BORDERS = [(2, (64, 64), 512, 32), (4, (128, 128), 128, 32), (3, (33, 65), 100, 20), (5, (17, 129), 72, 8), (2, (128, 128), 64, 1),
            (2, (40, 50), 1030, 2), (1, (300, 301), 48, 2), (16, (31, 33), 128, 32), (16, (32, 32), 128, 32), (8, (70, 71), 64, 8),
            (2, (9, 9), 2048, 4), (1, (200, 200), 5, 5), (40, (3, 5), 512, 512), (6, (90, 90), 96, 3), (2, (16, 16), 128, 2),
-           (2, (16, 16), 512, 1), (4, (15, 16), 256, 16)]
+           (2, (16, 16), 512, 1), (4, (15, 16), 256, 16),
+           (1, (4, 4), 512, 4), (1, (8, 8), 128, 2), (8, (8, 8), 256, 8), (8, (8, 9), 250, 5)]
 
 
 @pytest.mark.parametrize("dtype", sorted(K.TYPES))
