@@ -28,7 +28,7 @@
 //     207, 65       four waves, dealt out; operands read ahead
 //     201, 58       eight waves, two on a SIMD
 //     192, 58       f32: no branch in a step, no code decoded twice (this form)
-// f32: 1000 - 1070 TFLOP/s on the matrix cores (192 - 205 us, by the card), where a library's bf16 product of 8192^3 reaches 1217 on this card; the clock is what is left
+// f32: 990 - 1070 TFLOP/s on the matrix cores (192 - 208 us, by the card), where a library's bf16 product of 8192^3 reaches 1217 - 1362; the clock is what is left
 // (with gy = 0 the same launch takes 15 % less).  bf16: 45 us here and 12 in the kernel that adds the slices; of the 45, some 10 are
 // the first loads and the last stores.  65536 x 1024 x 2048 runs at 870 TFLOP/s.
 //

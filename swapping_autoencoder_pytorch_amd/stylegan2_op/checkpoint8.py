@@ -2,10 +2,11 @@
 its size, and the operators that read it there (csrc/checkpoint8.hip, csrc/linear_wgrad8.hip).
 
 The format (csrc/elem8.inc): blocks of 32 values along the last dimension with one power-of-two step each and a signed 8-bit code
-for each value; an error of at most half a step, 2^-8 ... 2^-7 of the block's largest value, where only a zero becomes zero (what
-is smaller than half a step becomes one step), so sign(x) is exact -- the mask that a leaky ReLU's backward reads.  (Next to the
-type's largest number, above 127.5 steps of the largest step, the error is up to one step.)  A block with a
-NaN or an infinity comes back as NaN.
+for each value.  A step is 1 / 127.5 ... 1 / 63.75 of the block's largest value (more where that is next to the smallest step, 2^-126,
+or 2^-24 in f16).  Values of at least half a step are off by half a step at most; what is smaller and not zero becomes one step, off
+by less than that, so that only a zero becomes zero and sign(x) is exact -- the mask that a leaky ReLU's backward reads.  (Next to
+the type's largest number, above 127.5 steps of the largest step, the error is up to one step.)  A block with a NaN or an infinity
+comes back as NaN.
 
   checkpoint8               activation -> Checkpoint8, ``.dequantize()`` gives it back
   linear_weight_grad8       weight and bias gradient of a linear layer from the Checkpoint8 of its input
@@ -236,7 +237,8 @@ def activation_checkpoints8(least=65536, enabled=True):
     8-bit checkpoints and gets them back when its backward runs, wherever that is; nodes that save the same tensor share one.  Parameters (trainable or frozen), other leaves
     that require a gradient, views of either, small, sparse and host tensors are kept as they are.  A weight that is no Parameter --
     detached, or computed from one -- is an activation here.  Forward values do not change; gradients are those at the values that
-    the checkpoints stand for."""
+    the checkpoints stand for.  In the backward pass a weight is known by its memory alone: convolutions inside lay it out anew for each
+    launch (``weight_prep``)."""
     if not enabled:
         yield
         return

@@ -81,7 +81,8 @@ def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, activati
     activation: "lrelu" (negative_slope; scale 2 ** 0.5 unless given, as ``fused_leaky_relu``), "silu" or "none" (scale 1 unless
     given).  x: float32, bfloat16 or float16, channels last in memory (any other order is copied into it); the result is channels
     last.  weight, bias: float32 [C] or None.  checkpoint: the backward pass works from the 8-bit checkpoint of x that the forward
-    writes beside y, instead of from x (``checkpoint8``); y is the same, the gradients are those at the values it stands for.
+    writes beside y, instead of from x (``checkpoint8``); y is the same but for the rounding of the statistics (rows are dealt out
+    to threads in whole blocks of 32 channels then), the gradients are those at the values it stands for.
     Differentiable once, in reverse mode."""
     if activation not in ACTIVATIONS:
         raise hip_lib.SaeError("group_norm_act: activation must be one of %s, got %r" % (sorted(ACTIVATIONS), activation))
@@ -107,7 +108,8 @@ def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, activati
 
 
 class GroupNormAct(nn.Module):
-    """``group_norm_act`` with its parameters (weight one, bias zero)."""
+    """``group_norm_act`` with its parameters (weight one, bias zero), which stay float32 for every type of input: convert the
+    activations, not the module."""
 
     def __init__(self, num_groups, channel, eps=1e-5, activation="lrelu", negative_slope=0.2, scale=None, checkpoint=False):
         super().__init__()
