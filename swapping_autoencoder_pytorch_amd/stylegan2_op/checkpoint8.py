@@ -234,11 +234,11 @@ def _unpack(k):
 @contextlib.contextmanager
 def activation_checkpoints8(least=65536, enabled=True):
     """Every autograd node built inside keeps the activations it saves (float32, bfloat16, float16; at least ``least`` values) as
-    8-bit checkpoints and gets them back when its backward runs, wherever that is; nodes that save the same tensor share one.  Parameters (trainable or frozen), other leaves
-    that require a gradient, views of either, small, sparse and host tensors are kept as they are.  A weight that is no Parameter --
-    detached, or computed from one -- is an activation here.  Forward values do not change; gradients are those at the values that
-    the checkpoints stand for.  In the backward pass a weight is known by its memory alone: convolutions inside lay it out anew for each
-    launch (``weight_prep``)."""
+    8-bit checkpoints and gets them back when its backward runs, wherever that is; nodes that save the same tensor share one.
+    Parameters (trainable or frozen), other leaves that require a gradient, views of either, small, sparse and host tensors are kept
+    as they are.  A weight that is no Parameter (a replica's, a detached or a computed one) is an activation here.  Forward values do
+    not change; gradients are those at the values that the checkpoints stand for.  In the backward pass a weight is known by its
+    memory alone: convolutions inside lay it out anew for each launch (``weight_prep``)."""
     if not enabled:
         yield
         return
