@@ -152,6 +152,8 @@ class Linear8(Function):
 def linear8(input, weight, bias=None, alpha=1.0):
     """``linear`` (alpha * input @ weight^T + bias, float32) whose backward takes the weight gradient from the 8-bit checkpoint of
     the input; y and the input gradient are ``linear``'s.  Differentiable once."""
+    if input.dim() < 1 or weight.dim() != 2:
+        raise hip_lib.SaeError("linear8: input [..., in] and weight [out, in], got %s and %s" % (tuple(input.shape), tuple(weight.shape)))
     lead = input.shape[:-1]
     x2 = input.reshape(-1, input.shape[-1])
     train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, bias))

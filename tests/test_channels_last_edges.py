@@ -209,10 +209,25 @@ def check_sizes_refused(device):
         lib.call("group_norm_act", p, None, None, p, p, p, None, None, 1, 1, 1, 1, -1.0, 0, 0.2, 1.0, 0, p, 64, None)
 
 
+def check_linear_refused(device):
+    """a bias of another length, which the kernel would read past its end, and tensors on two devices"""
+    x, w = K.seeded((6, 8), 1).to(device), K.seeded((5, 8), 2).to(device)
+    elsewhere = torch.empty(5, 8, device="meta")
+    for call in (ops.linear8, ops.linear):
+        for args in ((x, w, torch.zeros(4, device=device)), (x, w, torch.zeros(6, device=device)), (x, w, torch.zeros(1, device=device)),
+                     (x, w, torch.zeros(5, 5, device=device)), (x, elsewhere), (x, w, elsewhere[:, 0]), (x[:, :7], w), (x, w[:, :7])):
+            with pytest.raises(hip_lib.SaeError):
+                call(*args)
+        assert call(x, w, torch.zeros(5, device=device)).shape == (6, 5)
+    for args in ((torch.zeros((), device=device), w), (x, w[0]), (x, w[None])):
+        with pytest.raises(hip_lib.SaeError):
+            ops.linear8(*args)
+
+
 CHECKS = [check_frozen_parameters, check_forward_mode, check_negative_views, check_shared, check_linear8_bias_alone]
 
 
-@pytest.mark.parametrize("check", CHECKS + [check_other_layouts, check_sizes_refused], ids=lambda f: f.__name__[6:])
+@pytest.mark.parametrize("check", CHECKS + [check_other_layouts, check_sizes_refused, check_linear_refused], ids=lambda f: f.__name__[6:])
 def test_emulated(emu_lib, check):
     with backend(emu_lib):
         check("cpu")
